@@ -1406,6 +1406,22 @@ int fl_model_logits_nll(fl_model *m, int row0, int rows, const int32_t *next_tok
     (void)hipFree(out);
     return e == hipSuccess ? FL_OK : hip_fail(e, "fl_model_logits_nll");
 }
+/* fl_sample on the same rows */
+int fl_model_logits_sample(fl_model *m, int row0, int rows, const float *u_host, const fl_sample_params *p, int32_t *tokens_host) {
+    if (!m || !m->finalized || !u_host || !p || !tokens_host || row0 < 0 || rows < 1 || rows > m->B - row0)
+        return set_error(FL_EINVAL, "fl_model_logits_sample: bad argument");
+    float *u = nullptr;                                          // rows numbers, and the tokens behind them
+    M_HIP(hipMalloc((void **)&u, (size_t)rows * 8));
+    int32_t *out = reinterpret_cast<int32_t *>(u + rows);
+    int rc = FL_OK;
+    hipError_t e = hipMemcpyAsync(u, u_host, (size_t)rows * 4, hipMemcpyHostToDevice, m->stream);
+    if (e == hipSuccess) rc = fl_sample(FL_TYPE_F32, m->logits + (size_t)row0 * m->ldl, m->ldl, rows, m->V, u, p, out, m->stream);
+    if (e == hipSuccess && rc == FL_OK) e = hipMemcpyAsync(tokens_host, out, (size_t)rows * 4, hipMemcpyDeviceToHost, m->stream);
+    const hipError_t f = hipStreamSynchronize(m->stream);        // (also behind a failure: u_host and u are the stream's until then)
+    (void)hipFree(u);
+    if (rc != FL_OK) return rc;
+    return e != hipSuccess || f != hipSuccess ? hip_fail(e != hipSuccess ? e : f, "fl_model_logits_sample") : FL_OK;
+}
 void *fl_model_stream(const fl_model *m) { return m ? (void *)m->stream : nullptr; }
 size_t fl_model_device_bytes(const fl_model *m) { return m ? m->dev_bytes : 0; }
 

@@ -15,6 +15,8 @@ LIB_PATH = os.environ.get("FASTLLAMA_HIP_LIB") or os.path.join(PKG_DIR, "libfast
 
 FL_OK, FL_EINVAL, FL_EHIP, FL_ENOMEM, FL_ENODEV = 0, -1, -2, -3, -4
 Q4_0, Q4_1 = 2, 3
+F32, F16, BF16 = 0, 1, 30
+SAMPLE_MAX_VOCAB = 262144
 BLOCK_BYTES = {Q4_0: 20, Q4_1: 24}
 Q8_BLOCK_BYTES = 40
 QK = 32
@@ -40,6 +42,24 @@ class ModelParams(C.Structure):
     """fl_model_params"""
     _fields_ = [(n, C.c_int) for n in ("n_vocab", "n_embd", "n_head", "n_layer", "n_ff", "n_ctx", "qtype",
                                        "max_batch", "tp_rank", "tp_size")]
+
+
+class Heads(C.Structure):
+    """fl_heads"""
+    _fields_ = [("data_dev", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class KVPagesDesc(C.Structure):
+    """fl_kv_pages"""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("type", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_head_kv", C.c_int), ("head_dim", C.c_int), ("page_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("slot_stride", C.c_int64)]
+
+
+class SampleParams(C.Structure):
+    """fl_sample_params"""
+    _fields_ = [("temperature_dev", C.c_void_p), ("top_k_dev", C.c_void_p), ("top_p_dev", C.c_void_p), ("min_p_dev", C.c_void_p),
+                ("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("min_p", C.c_float)]
 
 
 _PROTOS = {
@@ -85,6 +105,15 @@ _PROTOS = {
     "fl_qact_export": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p]),
     "fl_mul_mat_q": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p]),
     "fl_mul_mat_q_f32": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p]),
+    "fl_kv_append": (C.c_int, [C.POINTER(KVPagesDesc), C.c_int, C.POINTER(Heads), C.POINTER(Heads), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
+                               C.c_int, C.c_int, C.c_int, C.c_void_p]),
+    "fl_attn_prompt": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.POINTER(Heads), C.c_int, C.POINTER(Heads), C.POINTER(Heads),
+                                 C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(Heads), C.c_void_p]),
+    "fl_attn_pages_workspace": (C.c_size_t, [C.POINTER(KVPagesDesc), C.c_int, C.c_int, C.c_int]),
+    "fl_attn_pages": (C.c_int, [C.POINTER(KVPagesDesc), C.c_int, C.c_float, C.POINTER(Heads), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
+                                C.c_int, C.c_int, C.POINTER(Heads), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fl_sample": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.POINTER(SampleParams), C.c_void_p, C.c_void_p]),
+    "fl_model_logits_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.POINTER(SampleParams), C.c_void_p]),
     "fl_comm_unique_id": (C.c_int, [C.c_void_p]),
     "fl_comm_create": (C.c_void_p, [C.c_void_p, C.c_int, C.c_int]),
     "fl_comm_create_local": (C.c_int, [C.c_int, C.POINTER(C.c_void_p)]),

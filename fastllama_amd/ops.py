@@ -9,6 +9,13 @@ Names and argument meaning follow the reference (``quantize_fns_t`` include/ggml
 * ``vec_dot_q``            quantize_fns[type].vec_dot_q
 * ``mul_mat``              ggml_mul_mat(W, x) for quantized W  ->  ggml_compute_forward_mul_mat_q_f32
 
+and the operators of a serving step over several sequences, which the reference does not have:
+
+* ``KVPages``              a paged K/V cache over tensors of the caller's; ``kv_append`` writes rows into it
+* ``attn_prompt``          causal attention with grouped heads over packed prompts
+* ``attn_pages``           the same over a paged cache: one new token for each sequence, or chunks of prompts
+* ``sample``               temperature / top-k / top-p / min-p from given uniform numbers
+
 torch is used only to own device memory and to pick the stream; every computation happens inside
 libfastllama_hip.so.  Nothing here computes on the CPU.
 """
@@ -177,4 +184,161 @@ def mul_mat_q(W: QTensor, a: QAct, which: int | None = None, out: torch.Tensor |
     else:
         check(lib.fl_debug_mul_mat_q(W.handle, a.handle, _dev(out), out.stride(0), which, _stream()),
               "fl_debug_mul_mat_q")
+    return out
+
+
+# ---- several sequences (fastllama_hip.h "several sequences": the formulas, limits and what is done with places outside the buffers) ----
+_TYPES = {torch.float32: hip.F32, torch.float16: hip.F16, torch.bfloat16: hip.BF16}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise hip.FastLlamaHipError(what)
+
+
+def _type(t: torch.Tensor, what: str) -> int:
+    _need(t.dtype in _TYPES, f"{what}: {t.dtype} is not float32, float16 or bfloat16")
+    return _TYPES[t.dtype]
+
+
+def _here(t: torch.Tensor, device: int, what: str) -> None:
+    """The kernels run on the current device's current stream."""
+    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{what}: expected a device tensor: fastllama_amd has no CPU path")
+    _need(t.get_device() == device, f"{what} is on {t.device}, the current device is cuda:{device}")
+
+
+def _heads(t: torch.Tensor, device: int, what: str) -> hip.Heads:
+    """[rows, heads, head_dim] of any strides, the last axis dense"""
+    _here(t, device, what)
+    _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{what}: want [rows, heads, head_dim] with a dense last axis, got {tuple(t.shape)} strides {t.stride()}")
+    n, h, _ = t.shape
+    return hip.Heads(t.data_ptr(), t.stride(0) if n > 1 else 0, t.stride(1) if h > 1 else 0)
+
+
+def _index(t: torch.Tensor, device: int, what: str, n: int) -> int:
+    _here(t, device, what)
+    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1), f"{what}: want {n} dense int32, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr()
+
+
+def _table(t: torch.Tensor, device: int) -> tuple[int, int]:
+    """(address, row stride) of [sequences, pages]"""
+    _here(t, device, "table")
+    _need(t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] < 2 or t.stride(1) == 1), f"table: want int32 [sequences, pages] with a dense last axis, got {tuple(t.shape)} {t.dtype}")
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+class KVPages:
+    """A paged K/V cache: ``k`` and ``v`` are [n_pages, n_head_kv, page_size, head_dim] views (any strides, the last axis dense, both alike) of
+    float32, float16 or bfloat16.  Position p of a sequence is slot p % page_size of page table[sequence][p // page_size]."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor):
+        for t, what in ((k, "k"), (v, "v")):
+            _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{what}: expected a device tensor: fastllama_amd has no CPU path")
+            _need(t.dim() == 4 and (t.stride(3) == 1 or t.shape[3] == 1), f"{what}: want [n_pages, n_head_kv, page_size, head_dim] with a dense last axis, got {tuple(t.shape)}")
+        _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device, "k and v are not alike")
+        strides = [tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)) for t in (k, v)]
+        _need(strides[0] == strides[1], "k and v have other strides")
+        self.k, self.v, self.device = k, v, k.get_device()
+        (n, h, p, d), (sp, sh, ss) = k.shape, strides[0]
+        self.desc = hip.KVPagesDesc(k.data_ptr(), v.data_ptr(), _type(k, "k"), n, p, h, d, sp, sh, ss)
+        self.ref = C.byref(self.desc)
+
+    @classmethod
+    def empty(cls, n_pages: int, page_size: int, n_head_kv: int, head_dim: int, dtype: torch.dtype = torch.float16) -> "KVPages":
+        shape = (n_pages, n_head_kv, page_size, head_dim)
+        return cls(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
+
+    def check(self, device: int) -> None:
+        _need(self.device == device, f"the cache is on cuda:{self.device}, the current device is cuda:{device}")
+
+
+def kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, n_past: torch.Tensor, cu: torch.Tensor | None = None) -> None:
+    """Rows ``k``, ``v`` [rows, n_head_kv, head_dim] (the cache's type, or float32: rounded once) become the positions behind n_past[b] of their
+    sequences: rows cu[b]..cu[b+1]-1, or one row for each sequence where cu is None.  No two rows of a call may go to one slot."""
+    device, d = torch.cuda.current_device(), pages.desc
+    pages.check(device)
+    _need(k.shape == v.shape and k.dtype == v.dtype and k.dim() == 3 and k.shape[1] == d.n_head_kv and k.shape[2] == d.head_dim,
+          f"k, v: want [rows, {d.n_head_kv}, {d.head_dim}] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
+    kh, vh, (tab, ld) = _heads(k, device, "k"), _heads(v, device, "v"), _table(table, device)
+    n = table.shape[0]
+    _need(cu is not None or n == k.shape[0], f"{k.shape[0]} rows for {n} sequences and no row starts")
+    check(hip.load().fl_kv_append(pages.ref, _type(k, "k"), C.byref(kh), C.byref(vh), k.shape[0], None if cu is None else _index(cu, device, "cu", n + 1),
+                                  _index(n_past, device, "n_past", n), tab, ld, table.shape[1], n, _stream()), "fl_kv_append")
+
+
+def _out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _need(out.shape == q.shape and out.dtype == q.dtype, f"out: want {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
+    return out
+
+
+def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_kv: torch.Tensor | None = None, scale: float | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of packed rows ``q`` [rows, n_head, head_dim] over ``k``, ``v`` [keys, n_head_kv, head_dim]; sequence b owns the rows
+    cu_q[b]..cu_q[b+1]-1 and the keys cu_kv[b]..cu_kv[b+1]-1 (None: as the rows).  The last row sees every key of its sequence, each row before it
+    one less; one that sees none becomes 0.  Rows outside every sequence are not written.  scale: 1 / sqrt(head_dim) unless given."""
+    device = torch.cuda.current_device()
+    qh, kh, vh = _heads(q, device, "q"), _heads(k, device, "k"), _heads(v, device, "v")
+    _need(k.shape == v.shape and k.shape[2] == q.shape[2] and q.dtype == k.dtype == v.dtype, f"q, k, v: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit together")
+    _here(cu_q, device, "cu_q")
+    n = cu_q.numel() - 1
+    _need(n >= 0 and (cu_kv is not None or q.shape[0] == k.shape[0]), "cu_q is empty, or other numbers of rows and keys and no cu_kv")
+    cu = _index(cu_q, device, "cu_q", n + 1)
+    out = _out(q, out)
+    oh = _heads(out, device, "out")
+    check(hip.load().fl_attn_prompt(_type(q, "q"), q.shape[2], q.shape[1], k.shape[1], q.shape[2] ** -0.5 if scale is None else scale, C.byref(qh), q.shape[0],
+                                    C.byref(kh), C.byref(vh), k.shape[0], cu, cu if cu_kv is None else _index(cu_kv, device, "cu_kv", n + 1), n, C.byref(oh),
+                                    _stream()), "fl_attn_prompt")
+    return out
+
+
+def attn_pages(q: torch.Tensor, pages: KVPages, table: torch.Tensor, kv_len: torch.Tensor, cu_q: torch.Tensor | None = None, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of ``q`` [rows, n_head, head_dim] over the first kv_len[b] positions of each sequence in the cache: one row for each
+    sequence (its newest token), or with ``cu_q`` the rows cu_q[b]..cu_q[b+1]-1 of each (its newest tokens, already in the cache)."""
+    device, d = torch.cuda.current_device(), pages.desc
+    pages.check(device)
+    qh, (tab, ld) = _heads(q, device, "q"), _table(table, device)
+    n = table.shape[0]
+    _need(q.dtype == pages.k.dtype and q.shape[2] == d.head_dim, f"q: {tuple(q.shape)} {q.dtype} does not fit a cache of head_dim {d.head_dim}, {pages.k.dtype}")
+    _need(cu_q is not None or n == q.shape[0], f"{q.shape[0]} rows for {n} sequences and no row starts")
+    lens, cu = _index(kv_len, device, "kv_len", n), None if cu_q is None else _index(cu_q, device, "cu_q", n + 1)
+    out = _out(q, out)
+    oh, lib = _heads(out, device, "out"), hip.load()
+    size = 0 if cu_q is not None else lib.fl_attn_pages_workspace(pages.ref, q.shape[1], table.shape[1], n)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    check(lib.fl_attn_pages(pages.ref, q.shape[1], d.head_dim ** -0.5 if scale is None else scale, C.byref(qh), q.shape[0], cu, lens, tab, ld, table.shape[1], n,
+                            C.byref(oh), ws.data_ptr() if size else None, size, _stream()), "fl_attn_pages")
+    return out
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """A token (int32 [rows]) for each row of ``logits`` [rows, n_vocab] from the uniform numbers ``u`` [rows] in [0, 1).  Each setting is a number
+    for all rows or a device tensor of one for each (float32; top_k int32).  Off: top_k <= 0, top_p >= 1, min_p <= 0; temperature <= 0 is greedy."""
+    device = torch.cuda.current_device()
+    _here(logits, device, "logits")
+    _need(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), f"logits: want [rows, n_vocab] with a dense last axis, got {tuple(logits.shape)}")
+    rows, vocab = logits.shape
+    p = hip.SampleParams()
+
+    def per_row(t, what, dtype):
+        _here(t, device, what)
+        _need(t.dtype == dtype and t.dim() == 1 and t.shape[0] == rows and (rows < 2 or t.stride(0) == 1), f"{what}: want {rows} dense {dtype}, got {tuple(t.shape)} {t.dtype}")
+        return t.data_ptr()
+
+    for what, x in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
+        if isinstance(x, torch.Tensor):
+            setattr(p, what + "_dev", per_row(x, what, torch.float32))
+        else:
+            setattr(p, what, x)
+    if isinstance(top_k, torch.Tensor):
+        p.top_k_dev = per_row(top_k, "top_k", torch.int32)
+    else:
+        p.top_k = max(0, min(int(top_k), vocab))
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    check(hip.load().fl_sample(_type(logits, "logits"), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, per_row(u, "u", torch.float32),
+                               C.byref(p), per_row(out, "out", torch.int32), _stream()), "fl_sample")
     return out

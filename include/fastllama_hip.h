@@ -37,6 +37,9 @@ extern "C" {
 
 #define FL_TYPE_Q4_0 2 /* enum ggml_type GGML_TYPE_Q4_0, include/ggml.h:200-212 */
 #define FL_TYPE_Q4_1 3 /* GGML_TYPE_Q4_1 */
+#define FL_TYPE_F32 0  /* GGML_TYPE_F32 */
+#define FL_TYPE_F16 1  /* GGML_TYPE_F16 */
+#define FL_TYPE_BF16 30 /* no type of the reference */
 
 /* ---------------------------------------------------------------- runtime ---------------------- */
 /* replaces: nothing in the reference (CPU only); hook point is FastLlama::Params::build,
@@ -149,6 +152,65 @@ int fl_mul_mat_q(const fl_qtensor *W, const fl_qact *a, float *y_dev, int ldy, v
  * grow-on-demand workspace (do not call while a hipGraph capture is active). */
 int fl_mul_mat_q_f32(const fl_qtensor *W, const float *x_dev, int ldx, float *y_dev, int ldy, int N, void *stream);
 
+/* ---------------------------------------------------------------- several sequences -------------- */
+/* Operators of a serving step over several sequences (fl_mul_mat_q_f32 projects their rows; these do the rest): new keys and values go
+ * into the pages of a cache, attention reads them, and a token is drawn for each row of logits.  New: the reference evaluates one
+ * sequence, with the attention of lib/llama.cpp:344-399 and the sampler of lib/bridge.cpp:24-108.
+ *
+ * Types: f32, f16, bf16; products, softmax statistics and sums are held in 32 bits (the sampler's in 64), outputs are rounded once.  In the
+ * 16-bit types the softmax's numerators are rounded to the type before they meet the values.  Heads: query head h reads key head
+ * h / (n_head / n_head_kv).  head_dim: a multiple of 8 up to 128.  Data and strides are multiples of 16 bytes; the last axis is dense.
+ *
+ * Sequences: row starts `cu` (n_seq + 1 of them, not falling), lengths, past positions and page numbers are DEVICE data, so a captured graph
+ * may be replayed on new ones.  Values that leave the buffers are cut, not reported: rows to those that exist, lengths to the table's
+ * n_table * page_size, and a page number outside 0..n_pages-1 stands for keys that are not there.  Rows outside every sequence are neither
+ * read nor written.  Every entry point launches on `stream`, allocates nothing, waits for nothing and may be captured. */
+typedef struct {
+    void *data_dev;                    /* element (row, head, d) at row * token_stride + head * head_stride + d */
+    int64_t token_stride, head_stride; /* in elements */
+} fl_heads;
+
+typedef struct {
+    void *k_dev, *v_dev;                            /* element (page, head, slot, d) at page * page_stride + head * head_stride + slot * slot_stride + d */
+    int type, n_pages, page_size, n_head_kv, head_dim; /* page_size: a power of two in 16..65536 */
+    int64_t page_stride, head_stride, slot_stride;  /* in elements, for keys and values alike */
+} fl_kv_pages;
+
+/* Row j of sequence b (k, v: n_tokens packed rows of src_type = f32 or the cache's type, rows cu[b]..cu[b+1]-1) becomes position n_past[b] + j
+ * of the cache: slot position % page_size of page table[b][position / page_size].  cu_dev NULL: one row for each sequence.  Positions without a
+ * page are not written.  No two rows of a call may go to one slot. */
+int fl_kv_append(const fl_kv_pages *c, int src_type, const fl_heads *k, const fl_heads *v, int n_tokens, const int32_t *cu_dev,
+                 const int32_t *n_past_dev, const int32_t *table_dev, int table_ld, int n_table, int n_seq, void *stream);
+/* Causal attention over packed prompts: rows cu_q[b].. of q see the keys cu_kv[b].. of their own sequence; the last row sees all of them and each row
+ * before it one less (more keys than rows: positions that were there before).  A row that sees no key becomes 0. */
+int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scale, const fl_heads *q, int n_q, const fl_heads *k, const fl_heads *v, int n_kv,
+                   const int32_t *cu_q_dev, const int32_t *cu_kv_dev, int n_seq, const fl_heads *out, void *stream);
+/* The same over a cache: sequence b has positions 0..kv_len[b]-1 in the pages table[b][...] (row stride table_ld, n_table pages each).  cu_q_dev
+ * NULL: one row for each sequence, the newest token; the work is split over long caches and joined, for which the caller keeps a workspace of
+ * fl_attn_pages_workspace() bytes (0: none) that no other call uses at the same time.  Otherwise cu_q gives the rows of each sequence, the
+ * newest kv_len[b] positions' last, and no workspace is used. */
+size_t fl_attn_pages_workspace(const fl_kv_pages *c, int n_head, int n_table, int n_seq);
+int fl_attn_pages(const fl_kv_pages *c, int n_head, float scale, const fl_heads *q, int n_q, const int32_t *cu_q_dev, const int32_t *kv_len_dev,
+                  const int32_t *table_dev, int table_ld, int n_table, int n_seq, const fl_heads *out, void *workspace_dev, size_t workspace_bytes,
+                  void *stream);
+
+/* One token for each row of logits l.  w_i = exp((l_i - max l) / temperature); in the order of (l falling, index rising) these are kept: the first
+ * top_k (<= 0: all); of them the shortest prefix whose sum is >= top_p times theirs (>= 1: all); of them those with w_i >= min_p (<= 0: all); the first
+ * always.  The token is the first kept index, in rising order, at which the running sum of the kept w exceeds u times their sum, u in [0, 1).
+ * temperature <= 0: the first index of the largest logit.  NaN counts as -infinity; a row of nothing else gives -1; logits of +infinity share the weight.
+ * The w are held in 2^-44 units (a token below that never comes up), sums of them are exact.  A *_dev pointer gives each row its own setting, NULL
+ * the scalar beside it to all. */
+#define FL_SAMPLE_MAX_VOCAB 262144
+typedef struct {
+    const float *temperature_dev;
+    const int32_t *top_k_dev;
+    const float *top_p_dev, *min_p_dev;
+    float temperature;
+    int top_k;
+    float top_p, min_p;
+} fl_sample_params;
+int fl_sample(int type, const void *logits_dev, int64_t ld, int rows, int n_vocab, const float *u_dev, const fl_sample_params *p, int32_t *tokens_dev,
+              void *stream);
 
 /* ---------------------------------------------------------------- collectives (RCCL over xGMI) -- */
 /* New for SURVEY.md section 8(e): the reference is single-process.  One process per GPU; rank 0 creates
@@ -275,6 +337,9 @@ int fl_model_logits_ld(const fl_model *m);
 int fl_model_logits_read(fl_model *m, int row0, int rows, float *logits_host);
 /* -log softmax(logits[row0 + i])[next_tokens_host[i]] on the device (FastLlama::perplexity's row loop, lib/bridge.cpp:397-407) */
 int fl_model_logits_nll(fl_model *m, int row0, int rows, const int32_t *next_tokens_host, double *nll_host);
+/* fl_sample on rows of the last eval's logits, on the device: tokens_host[i] for row row0 + i and the uniform number u_host[i]; rows * 4 bytes come
+ * back instead of the rows' logits.  p's *_dev pointers are NULL here or device data of `rows` values. */
+int fl_model_logits_sample(fl_model *m, int row0, int rows, const float *u_host, const fl_sample_params *p, int32_t *tokens_host);
 void *fl_model_stream(const fl_model *m);
 size_t fl_model_device_bytes(const fl_model *m);
 int fl_model_kv_read(const fl_model *m, float *k_host, float *v_host);
