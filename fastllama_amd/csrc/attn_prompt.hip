@@ -2,24 +2,89 @@
 //
 //   out[i][h] = sum_j exp(s_ij - max) v_j / sum_j exp(s_ij - max),  s_ij = scale q_i . k_j,  keys j <= lk - lq + i of i's own sequence
 //
-// First form: one wave for a row and head, a lane for a key; the maximum and sum run along (one pass over K and V).
+// The query heads that share a key head are rows of one problem: row r of (sequence, key head) is token r / group, head r % group, so a
+// workgroup's 128 rows read each key and value once for the whole group, and few tokens still fill a tile.  A wave has 32 rows; K and V pass
+// through LDS in tiles of KT keys, the next tile's loads in flight (registers) while this one is computed, two LDS tiles in turn: one barrier a tile.
+//
+// Both products are taken transposed: S^T = K Q^T leaves each lane a column, one query row with half of the tile's keys (lane and lane + 32
+// share the row), so maximum and sum run inside a lane; and its registers are, in their order, the operand P^T of O^T = V^T P^T, whose
+// columns are query rows again: the rescaling factor is a lane's own.  V^T comes out of LDS by transposing reads.
+//
+// The softmax's reference is not the running maximum but a value at most 2^8 below it: the accumulators are rescaled only when the maximum
+// has moved by more (p <= 2^8 fits f16 and costs no precision).  p is rounded to the inputs' type for the second product (the error of a
+// weighted mean of values that are themselves of that type); scores, sums and outputs are f32 until the one rounding at the end.
 #include "serve_kernels.h"
 #include "serve_device.h"
 #include "../../include/fastllama_hip.h"
 
 namespace fl {
 
-template <typename T, bool PAGED>
-__global__ __launch_bounds__(256) void attn_rows_k(AttnArgs a, bool decode) {
-    const int lane = threadIdx.x & 63, head = blockIdx.y, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.n_q) return;
-    int b = -1, q0 = 0, q1 = 0;
-    if (decode) b = row, q0 = row, q1 = row + 1;
-    else
-        for (int s = 0; s < a.n_seq; ++s) {
-            seq_rows(a.cu_q, s, a.n_q, &q0, &q1);
-            if (row >= q0 && row < q1) { b = s; break; }
+constexpr int PR_ROWS = 128;             // rows of a workgroup: 4 waves of 32
+
+template <typename T>
+struct Tile {                            // LDS tiles of a type
+    static constexpr int KT = sizeof(T) == 2 ? 64 : 32, KPAD = 16 / sizeof(T), VPAD = sizeof(T) == 2 ? 32 : 4;
+};
+
+// Four keys 4 * (lane / 32) + 0..3 and four more 8 behind them, of the 16 that start at `row`, at component d0 + lane % 32: the transposed operand.
+template <typename T, int LD>
+__device__ inline typename Vec<T>::x8 read_vt(const T *v, int row, int d0, int lane) {
+    typename Vec<T>::x8 r;
+    const int h = lane >> 5;
+    if constexpr (sizeof(T) == 2) {
+        // each group of 16 lanes reads 4 keys x 16 components, 4 components a lane, and gets them transposed
+        const int L = lane & 15;
+        const T *p = v + (row + 4 * h + (L >> 2)) * LD + d0 + ((lane >> 4) & 1) * 16 + 4 * (L & 3);
+        typedef __attribute__((address_space(3))) s16x4 *lds_p;
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 8 * LD));
+        typedef short s16x8 __attribute__((ext_vector_type(8)));
+        r = __builtin_bit_cast(typename Vec<T>::x8, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+        const T *p = v + (row + 4 * h) * LD + d0 + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = p[(i < 4 ? i : i + 4) * LD];
+    }
+    return r;
+}
+
+template <typename T, int DP, bool PAGED>
+__global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int KT = Tile<T>::KT, KLD = DP + Tile<T>::KPAD, VLD = DP + Tile<T>::VPAD;
+    constexpr int UNIT = 16 / sizeof(T), CPR = DP / UNIT, RPP = 256 / CPR, PASSES = KT / RPP;   // 16-byte chunks of a row, rows of a pass over the tile
+    constexpr int KB = KT / 32, DB = DP / 32, DS = DP / 16;
+    static_assert(KT % RPP == 0 && PASSES >= 1, "a tile is whole passes of the workgroup");
+    __shared__ __attribute__((aligned(16))) T ks[2][KT * KLD], vs[2][KT * VLD];
+
+    __shared__ int odd;
+    if (threadIdx.x == 0) odd = 0;
+    __syncthreads();
+
+    const int t = threadIdx.x, lane = t & 63, h = lane >> 5, n_head_kv = a.n_head / a.group;
+    // workgroups go round the 8 XCDs by their number: with 8 key heads (or a multiple) all that read a head's keys share an L2; the blocks with most keys first
+    const int hk = blockIdx.x % n_head_kv;
+    int blk = gridDim.x / n_head_kv - 1 - blockIdx.x / n_head_kv;
+
+    // the sequence that has block `blk` of all sequences' blocks: every wave scans 64 sequences at a time
+    int b = -1, q0 = 0, lq = 0;
+    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
+        int f = 0, e = 0;
+        if (s0 + lane < a.n_seq) seq_rows(a.cu_q, s0 + lane, a.n_q, &f, &e);
+        const int n = (int)(((int64_t)(e - f) * a.group + PR_ROWS - 1) / PR_ROWS);
+        int incl = n;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int up = __shfl_up(incl, o);
+            if (lane >= o) incl += up;
         }
+        const int total = __shfl(incl, 63);
+        if (blk < total) {
+            const int w = __ffsll((unsigned long long)__ballot(incl > blk)) - 1;
+            b = s0 + w, q0 = __shfl(f, w), lq = __shfl(e, w) - q0, blk -= __shfl(incl - n, w);
+            break;
+        }
+        blk -= total;
+    }
     if (b < 0) return;
     int k0 = 0, lk;
     if (PAGED) lk = (int)min((int64_t)max(a.kv_len[b], 0), (int64_t)a.n_table << a.page_shift);
@@ -28,63 +93,194 @@ __global__ __launch_bounds__(256) void attn_rows_k(AttnArgs a, bool decode) {
         seq_rows(a.cu_kv, b, a.n_kv, &k0, &k1);
         lk = k1 - k0;
     }
-    const int seen = min(lk, lk - (q1 - q0) + (row - q0) + 1);
-    const int D = a.head_dim, hk = head / a.group;
-    const T *q = (const T *)a.q + row * a.q_ld + head * a.q_hs;
-    float m = -INFINITY, l = 0, o0 = 0, o1 = 0;
-    for (int j0 = 0; j0 < seen; j0 += 64) {
-        const int j = j0 + lane;
-        int64_t ko = 0, vo = 0;
-        bool in = j < seen;
-        if (PAGED) {
-            const int pg = in ? a.table[(int64_t)b * a.table_ld + (j >> a.page_shift)] : -1;
-            in = in && pg >= 0 && pg < a.n_pages;
-            ko = vo = (in ? pg : 0) * a.page_stride + (j & ((1 << a.page_shift) - 1)) * a.k_ld;
-        } else ko = (in ? k0 + j : 0) * a.k_ld, vo = (in ? k0 + j : 0) * a.v_ld;
-        float s = -INFINITY;
-        if (in) {
-            const T *k = (const T *)a.k + ko + hk * a.k_hs;
-            s = 0;
-            for (int d = 0; d < D; ++d) s = fmaf((float)q[d], (float)k[d], s);
-            s *= a.scale_log2;
-        }
-        float mx = s;
-        for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        const float c = exp2f(m - ref), p = exp2f(s - ref);
-        float ps = p;
-        for (int o = 32; o; o >>= 1) ps += __shfl_xor(ps, o);
-        l = l * c + ps, o0 *= c, o1 *= c, m = mn;
-        const unsigned long long live = __ballot(in);
-        for (int t = 0; t < 64; ++t) {
-            if (!(live >> t & 1)) continue;
-            const float pt = __shfl(p, t);
-            const T *v = (const T *)a.v + __shfl(vo, t) + hk * a.v_hs;
-            if (lane < D) o0 = fmaf(pt, (float)v[lane], o0);
-            if (lane + 64 < D) o1 = fmaf(pt, (float)v[lane + 64], o1);
+    const int D = a.head_dim, rows = lq * a.group, r0 = blk * PR_ROWS, rw = r0 + (t >> 6) * 32, row = rw + (lane & 31);
+    const bool valid = row < rows;
+    const int tok = (valid ? row : rows - 1) / a.group, head = hk * a.group + (valid ? row : rows - 1) % a.group;
+    const int past = lk - lq, lim = past + tok;                    // the last key that this lane's row sees
+    const int lim_first = past + min(rw, rows - 1) / a.group, lim_last = past + min(rw + 31, rows - 1) / a.group;   // of the wave's rows
+    const int end = min(past + min(r0 + PR_ROWS - 1, rows - 1) / a.group + 1, lk), tiles = end > 0 ? (end + KT - 1) / KT : 0;
+
+    x8 qf[DS];
+    {
+        const T *q = (const T *)a.q + (int64_t)(q0 + tok) * a.q_ld + head * a.q_hs;
+#pragma unroll
+        for (int s = 0; s < DS; ++s) {
+            const int d = 16 * s + 8 * h;
+            qf[s] = valid && d < D ? *(const x8 *)(q + d) : (x8)(T)0;
         }
     }
-    T *o = (T *)a.out + row * a.o_ld + head * a.o_hs;
-    const float r = l > 0 || l != l ? 1 / l : 0.f;
-    if (lane < D) o[lane] = (T)(o0 * r);
-    if (lane + 64 < D) o[lane + 64] = (T)(o1 * r);
+
+    // this thread's part of a tile: chunk c of rows pr + RPP * p
+    const int c = (t % CPR) * UNIT, pr = t / CPR;
+    const T *kbase = (const T *)a.k + hk * a.k_hs + c, *vbase = (const T *)a.v + hk * a.v_hs + c;
+    const int32_t *table = PAGED ? a.table + (int64_t)b * a.table_ld : nullptr;
+    const int smask = (1 << a.page_shift) - 1;
+    u32x4 kr[PASSES], vr[PASSES];
+    int pg[PASSES];
+    uint32_t there = ~0u, there_next = ~0u;       // pages: a bit for each 16 keys of the tile that have a page
+    auto pages = [&](int tile) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int j = tile * KT + pr + RPP * p;
+            pg[p] = j < end ? table[j >> a.page_shift] : -1;
+        }
+    };
+    auto load = [&](int tile) {
+        if (PAGED) {
+            const int j = tile * KT + 16 * (lane & 3);
+            const int p = j < end ? table[j >> a.page_shift] : 0;
+            there_next = (uint32_t)__ballot(lane < KT / 16 && p >= 0 && p < a.n_pages);
+        }
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            const int j = tile * KT + pr + RPP * p;
+            bool in = j < end && c < D;
+            int64_t ko, vo;
+            if (PAGED) {
+                in = in && pg[p] >= 0 && pg[p] < a.n_pages;
+                ko = vo = (int64_t)pg[p] * a.page_stride + (j & smask) * a.k_ld;
+            } else ko = (int64_t)(k0 + j) * a.k_ld, vo = (int64_t)(k0 + j) * a.v_ld;
+            kr[p] = vr[p] = (u32x4)0u;
+            if (in) kr[p] = *(const u32x4 *)(kbase + ko), vr[p] = *(const u32x4 *)(vbase + vo);
+        }
+        if (PAGED) pages(tile + 1);
+    };
+    // A value that is not finite may not reach a row that does not see it, and 0 times it is not 0: in the tiles that some row of the workgroup sees
+    // in part it is stored as 0, and put back at the end for the rows that do see it.
+    const int whole = past + min(r0, rows - 1) / a.group + 1;      // every row sees the keys before this one
+    auto store = [&](int buf, int tile) {
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
+            if ((tile + 1) * KT > whole) {
+                typedef T xu __attribute__((ext_vector_type(UNIT)));
+                xu v = __builtin_bit_cast(xu, vr[p]);
+                bool any = false;
+#pragma unroll
+                for (int e = 0; e < UNIT; ++e) {
+                    any |= !finite(v[e]);
+                    v[e] = finite(v[e]) ? v[e] : (T)0.f;
+                }
+                if (any) odd = 1;
+                vr[p] = __builtin_bit_cast(u32x4, v);
+            }
+            *(u32x4 *)(ks[buf] + (pr + RPP * p) * KLD + c) = kr[p];
+            *(u32x4 *)(vs[buf] + (pr + RPP * p) * VLD + c) = vr[p];
+        }
+    };
+
+    f32x16 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = (f32x16)0.f;
+    float m = -INFINITY, l = 0;
+    if (PAGED) pages(0);
+    if (tiles) {
+        load(0);
+        store(0, 0);
+        there = there_next;
+    }
+    for (int tile = 0; tile < tiles; ++tile) {
+        const int buf = tile & 1, kv = tile * KT;
+        __syncthreads();
+        if (tile + 1 < tiles) load(tile + 1);
+        if (kv <= lim_last) {
+            f32x16 s[KB];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) s[kb] = (f32x16)0.f;
+#pragma unroll
+            for (int st = 0; st < DS; ++st)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) s[kb] = mfma32(*(const x8 *)(ks[buf] + (32 * kb + (lane & 31)) * KLD + 16 * st + 8 * h), qf[st], s[kb]);
+            const bool masked = kv + KT - 1 > lim_first || (PAGED && (there & ((1u << (KT / 16)) - 1)) != (1u << (KT / 16)) - 1);
+            auto seen = [&](int kb, int r) {              // register r of block kb: key 32 kb + 8 (r / 4) + 4 h + r % 4
+                return kv + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3) <= lim && (!PAGED || (there >> (2 * kb + (r >> 3)) & 1));
+            };
+            if (masked)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s[kb][r] = seen(kb, r) ? s[kb][r] : -INFINITY;
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+            mx = max_halves(mx) * a.scale_log2;
+            if (__any(mx > m + 8.f)) {
+                const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+                m = mn, l *= f;
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] *= f;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;
+            x8 p[KB][2];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.scale_log2, -ref));
+                    l += e;
+                    p[kb][r >> 3][r & 7] = (T)e;
+                }
+#pragma unroll
+            for (int i = 0; i < 2 * KB; ++i)
+#pragma unroll
+                for (int d = 0; d < DB; ++d) o[d] = mfma32(read_vt<T, VLD>(vs[buf], 16 * i, 32 * d, lane), p[i >> 1][i & 1], o[d]);
+        }
+        if (tile + 1 < tiles) {
+            store(buf ^ 1, tile + 1);
+            there = there_next;
+        }
+    }
+    l = sum_halves(l);
+    if (!valid) return;
+    const float inv = l == 0 ? 0.f : 1 / l;
+    if (tiles && odd)
+        for (int j = max(whole, 0) / KT * KT; j <= min(lim, end - 1); ++j) {
+            int64_t vo = (int64_t)(k0 + j) * a.v_ld;
+            if (PAGED) {
+                const int p = table[j >> a.page_shift];
+                if (p < 0 || p >= a.n_pages) continue;
+                vo = p * a.page_stride + (j & smask) * a.v_ld;
+            }
+            const T *v = (const T *)a.v + vo + hk * a.v_hs;
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int at = 32 * d + 8 * (r >> 2) + 4 * h + (r & 3);
+                    if (at < D && !finite(v[at])) o[d][r] += (float)v[at];
+                }
+        }
+    T *out = (T *)a.out + (int64_t)(q0 + tok) * a.o_ld + head * a.o_hs;
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            typedef T x4 __attribute__((ext_vector_type(4)));
+            const int at = 32 * d + 2 * r + 4 * h;
+            const f32x4 y = {o[d][r] * inv, o[d][r + 1] * inv, o[d][r + 2] * inv, o[d][r + 3] * inv};
+            if (at < D) *(x4 *)(out + at) = __builtin_convertvector(y, x4);
+        }
 }
 
-template <bool PAGED>
-static hipError_t rows_launch(const AttnArgs &a, int type, bool decode, hipStream_t st) {
-    const dim3 g((a.n_q + 3) / 4, a.n_head);
-    switch (type) {
-        case FL_TYPE_F32: attn_rows_k<float, PAGED><<<g, 256, 0, st>>>(a, decode); break;
-        case FL_TYPE_F16: attn_rows_k<h16, PAGED><<<g, 256, 0, st>>>(a, decode); break;
-        default: attn_rows_k<b16, PAGED><<<g, 256, 0, st>>>(a, decode); break;
-    }
+template <typename T, bool PAGED>
+static hipError_t prompt_launch(const AttnArgs &a, hipStream_t st) {
+    const int n_head_kv = a.n_head / a.group;
+    const int64_t blocks = ((int64_t)a.n_q * a.group / PR_ROWS + a.n_seq) * n_head_kv;   // every sequence may end inside a block
+    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 g((unsigned)blocks);
+    if (a.head_dim <= 32) attn_prompt_k<T, 32, PAGED><<<g, 256, 0, st>>>(a);
+    else if (a.head_dim <= 64) attn_prompt_k<T, 64, PAGED><<<g, 256, 0, st>>>(a);
+    else attn_prompt_k<T, 128, PAGED><<<g, 256, 0, st>>>(a);
     return hipGetLastError();
 }
 
 hipError_t attn_prompt(const AttnArgs &a, int type, bool paged, hipStream_t st) {
-    return paged ? rows_launch<true>(a, type, false, st) : rows_launch<false>(a, type, false, st);
+    switch (type) {
+        case FL_TYPE_F32: return paged ? prompt_launch<float, true>(a, st) : prompt_launch<float, false>(a, st);
+        case FL_TYPE_F16: return paged ? prompt_launch<h16, true>(a, st) : prompt_launch<h16, false>(a, st);
+        default: return paged ? prompt_launch<b16, true>(a, st) : prompt_launch<b16, false>(a, st);
+    }
 }
-hipError_t attn_decode(const AttnArgs &a, int type, hipStream_t st) { return rows_launch<true>(a, type, true, st); }
-size_t attn_decode_workspace(int, int, int, int, int64_t) { return 0; }
 
 }  // namespace fl

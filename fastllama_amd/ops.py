@@ -188,43 +188,45 @@ def mul_mat_q(W: QTensor, a: QAct, which: int | None = None, out: torch.Tensor |
 
 
 # ---- several sequences (fastllama_hip.h "several sequences": the formulas, limits and what is done with places outside the buffers) ----
+_Error = hip.FastLlamaHipError
 _TYPES = {torch.float32: hip.F32, torch.float16: hip.F16, torch.bfloat16: hip.BF16}
 
 
-def _need(ok: bool, what: str) -> None:
-    if not ok:
-        raise hip.FastLlamaHipError(what)
-
-
 def _type(t: torch.Tensor, what: str) -> int:
-    _need(t.dtype in _TYPES, f"{what}: {t.dtype} is not float32, float16 or bfloat16")
+    if not (t.dtype in _TYPES):
+        raise _Error(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
     return _TYPES[t.dtype]
 
 
 def _here(t: torch.Tensor, device: int, what: str) -> None:
     """The kernels run on the current device's current stream."""
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{what}: expected a device tensor: fastllama_amd has no CPU path")
-    _need(t.get_device() == device, f"{what} is on {t.device}, the current device is cuda:{device}")
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise _Error(f"{what}: expected a device tensor: fastllama_amd has no CPU path")
+    if not (t.get_device() == device):
+        raise _Error(f"{what} is on {t.device}, the current device is cuda:{device}")
 
 
 def _heads(t: torch.Tensor, device: int, what: str) -> hip.Heads:
     """[rows, heads, head_dim] of any strides, the last axis dense"""
     _here(t, device, what)
-    _need(t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1), f"{what}: want [rows, heads, head_dim] with a dense last axis, got {tuple(t.shape)} strides {t.stride()}")
+    if not (t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1)):
+        raise _Error(f"{what}: want [rows, heads, head_dim] with a dense last axis, got {tuple(t.shape)} strides {t.stride()}")
     n, h, _ = t.shape
     return hip.Heads(t.data_ptr(), t.stride(0) if n > 1 else 0, t.stride(1) if h > 1 else 0)
 
 
 def _index(t: torch.Tensor, device: int, what: str, n: int) -> int:
     _here(t, device, what)
-    _need(t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1), f"{what}: want {n} dense int32, got {tuple(t.shape)} {t.dtype}")
+    if not (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1)):
+        raise _Error(f"{what}: want {n} dense int32, got {tuple(t.shape)} {t.dtype}")
     return t.data_ptr()
 
 
 def _table(t: torch.Tensor, device: int) -> tuple[int, int]:
     """(address, row stride) of [sequences, pages]"""
     _here(t, device, "table")
-    _need(t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] < 2 or t.stride(1) == 1), f"table: want int32 [sequences, pages] with a dense last axis, got {tuple(t.shape)} {t.dtype}")
+    if not (t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] < 2 or t.stride(1) == 1)):
+        raise _Error(f"table: want int32 [sequences, pages] with a dense last axis, got {tuple(t.shape)} {t.dtype}")
     return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
@@ -234,11 +236,15 @@ class KVPages:
 
     def __init__(self, k: torch.Tensor, v: torch.Tensor):
         for t, what in ((k, "k"), (v, "v")):
-            _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{what}: expected a device tensor: fastllama_amd has no CPU path")
-            _need(t.dim() == 4 and (t.stride(3) == 1 or t.shape[3] == 1), f"{what}: want [n_pages, n_head_kv, page_size, head_dim] with a dense last axis, got {tuple(t.shape)}")
-        _need(k.shape == v.shape and k.dtype == v.dtype and k.device == v.device, "k and v are not alike")
+            if not (isinstance(t, torch.Tensor) and t.is_cuda):
+                raise _Error(f"{what}: expected a device tensor: fastllama_amd has no CPU path")
+            if not (t.dim() == 4 and (t.stride(3) == 1 or t.shape[3] == 1)):
+                raise _Error(f"{what}: want [n_pages, n_head_kv, page_size, head_dim] with a dense last axis, got {tuple(t.shape)}")
+        if not (k.shape == v.shape and k.dtype == v.dtype and k.device == v.device):
+            raise _Error("k and v are not alike")
         strides = [tuple(t.stride(i) if t.shape[i] > 1 else 0 for i in range(3)) for t in (k, v)]
-        _need(strides[0] == strides[1], "k and v have other strides")
+        if not (strides[0] == strides[1]):
+            raise _Error("k and v have other strides")
         self.k, self.v, self.device = k, v, k.get_device()
         (n, h, p, d), (sp, sh, ss) = k.shape, strides[0]
         self.desc = hip.KVPagesDesc(k.data_ptr(), v.data_ptr(), _type(k, "k"), n, p, h, d, sp, sh, ss)
@@ -250,7 +256,8 @@ class KVPages:
         return cls(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
 
     def check(self, device: int) -> None:
-        _need(self.device == device, f"the cache is on cuda:{self.device}, the current device is cuda:{device}")
+        if not (self.device == device):
+            raise _Error(f"the cache is on cuda:{self.device}, the current device is cuda:{device}")
 
 
 def kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, n_past: torch.Tensor, cu: torch.Tensor | None = None) -> None:
@@ -258,11 +265,12 @@ def kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     sequences: rows cu[b]..cu[b+1]-1, or one row for each sequence where cu is None.  No two rows of a call may go to one slot."""
     device, d = torch.cuda.current_device(), pages.desc
     pages.check(device)
-    _need(k.shape == v.shape and k.dtype == v.dtype and k.dim() == 3 and k.shape[1] == d.n_head_kv and k.shape[2] == d.head_dim,
-          f"k, v: want [rows, {d.n_head_kv}, {d.head_dim}] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
+    if not (k.shape == v.shape and k.dtype == v.dtype and k.dim() == 3 and k.shape[1] == d.n_head_kv and k.shape[2] == d.head_dim):
+        raise _Error(f"k, v: want [rows, {d.n_head_kv}, {d.head_dim}] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
     kh, vh, (tab, ld) = _heads(k, device, "k"), _heads(v, device, "v"), _table(table, device)
     n = table.shape[0]
-    _need(cu is not None or n == k.shape[0], f"{k.shape[0]} rows for {n} sequences and no row starts")
+    if not (cu is not None or n == k.shape[0]):
+        raise _Error(f"{k.shape[0]} rows for {n} sequences and no row starts")
     check(hip.load().fl_kv_append(pages.ref, _type(k, "k"), C.byref(kh), C.byref(vh), k.shape[0], None if cu is None else _index(cu, device, "cu", n + 1),
                                   _index(n_past, device, "n_past", n), tab, ld, table.shape[1], n, _stream()), "fl_kv_append")
 
@@ -270,7 +278,8 @@ def kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
 def _out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _need(out.shape == q.shape and out.dtype == q.dtype, f"out: want {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
+    if not (out.shape == q.shape and out.dtype == q.dtype):
+        raise _Error(f"out: want {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
     return out
 
 
@@ -281,10 +290,12 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     one less; one that sees none becomes 0.  Rows outside every sequence are not written.  scale: 1 / sqrt(head_dim) unless given."""
     device = torch.cuda.current_device()
     qh, kh, vh = _heads(q, device, "q"), _heads(k, device, "k"), _heads(v, device, "v")
-    _need(k.shape == v.shape and k.shape[2] == q.shape[2] and q.dtype == k.dtype == v.dtype, f"q, k, v: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit together")
+    if not (k.shape == v.shape and k.shape[2] == q.shape[2] and q.dtype == k.dtype == v.dtype):
+        raise _Error(f"q, k, v: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit together")
     _here(cu_q, device, "cu_q")
     n = cu_q.numel() - 1
-    _need(n >= 0 and (cu_kv is not None or q.shape[0] == k.shape[0]), "cu_q is empty, or other numbers of rows and keys and no cu_kv")
+    if not (n >= 0 and (cu_kv is not None or q.shape[0] == k.shape[0])):
+        raise _Error("cu_q is empty, or other numbers of rows and keys and no cu_kv")
     cu = _index(cu_q, device, "cu_q", n + 1)
     out = _out(q, out)
     oh = _heads(out, device, "out")
@@ -302,8 +313,10 @@ def attn_pages(q: torch.Tensor, pages: KVPages, table: torch.Tensor, kv_len: tor
     pages.check(device)
     qh, (tab, ld) = _heads(q, device, "q"), _table(table, device)
     n = table.shape[0]
-    _need(q.dtype == pages.k.dtype and q.shape[2] == d.head_dim, f"q: {tuple(q.shape)} {q.dtype} does not fit a cache of head_dim {d.head_dim}, {pages.k.dtype}")
-    _need(cu_q is not None or n == q.shape[0], f"{q.shape[0]} rows for {n} sequences and no row starts")
+    if not (q.dtype == pages.k.dtype and q.shape[2] == d.head_dim):
+        raise _Error(f"q: {tuple(q.shape)} {q.dtype} does not fit a cache of head_dim {d.head_dim}, {pages.k.dtype}")
+    if not (cu_q is not None or n == q.shape[0]):
+        raise _Error(f"{q.shape[0]} rows for {n} sequences and no row starts")
     lens, cu = _index(kv_len, device, "kv_len", n), None if cu_q is None else _index(cu_q, device, "cu_q", n + 1)
     out = _out(q, out)
     oh, lib = _heads(out, device, "out"), hip.load()
@@ -319,13 +332,15 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     for all rows or a device tensor of one for each (float32; top_k int32).  Off: top_k <= 0, top_p >= 1, min_p <= 0; temperature <= 0 is greedy."""
     device = torch.cuda.current_device()
     _here(logits, device, "logits")
-    _need(logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1), f"logits: want [rows, n_vocab] with a dense last axis, got {tuple(logits.shape)}")
+    if not (logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
+        raise _Error(f"logits: want [rows, n_vocab] with a dense last axis, got {tuple(logits.shape)}")
     rows, vocab = logits.shape
     p = hip.SampleParams()
 
     def per_row(t, what, dtype):
         _here(t, device, what)
-        _need(t.dtype == dtype and t.dim() == 1 and t.shape[0] == rows and (rows < 2 or t.stride(0) == 1), f"{what}: want {rows} dense {dtype}, got {tuple(t.shape)} {t.dtype}")
+        if not (t.dtype == dtype and t.dim() == 1 and t.shape[0] == rows and (rows < 2 or t.stride(0) == 1)):
+            raise _Error(f"{what}: want {rows} dense {dtype}, got {tuple(t.shape)} {t.dtype}")
         return t.data_ptr()
 
     for what, x in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
