@@ -1,84 +1,286 @@
 // attn_decode.hip -- attention of one new token for each sequence over a paged cache.
 //
-//   out[i][h] = sum_j exp(s_ij - max) v_j / sum_j exp(s_ij - max),  s_ij = scale q_i . k_j,  keys j <= lk - lq + i of i's own sequence
+//   out[b][h] = sum_j exp(s_j - max) v_j / sum_j exp(s_j - max),  s_j = scale q . k_j,  j < kv_len[b]
 //
-// First form: one wave for a row and head, a lane for a key; the maximum and sum run along (one pass over K and V).
+// Bound by reading K and V once.  The query heads of a key head (16 at most at a time) are the columns of one small problem on the matrix units;
+// with one query head 15 of 16 columns are idle, which costs nothing that is missed: the reads still take longer.  Both products are taken
+// transposed (attn_prompt.hip): S^T = K Q^T, O^T = V^T P^T, so K goes from memory straight into its operand's registers, P stays where S was
+// made, and V alone passes through LDS, each wave by itself: there is no barrier before the end.  A wave has the next tile's K and V in flight
+// while it works on this one.
+//
+// A sequence's keys are cut into chunks; a workgroup's four waves take every fourth tile of a chunk and join their maxima, sums and outputs in LDS.
+// A sequence of one chunk is done then; the chunks of a longer one leave theirs in the workspace for a second launch to join.  Chunks are
+// of one length, so the work of a ragged batch is even, and workgroups behind a sequence's end leave at once.
 #include "serve_kernels.h"
 #include "serve_device.h"
 #include "../../include/fastllama_hip.h"
 
 namespace fl {
 
-template <typename T, bool PAGED>
-__global__ __launch_bounds__(256) void attn_rows_k(AttnArgs a, bool decode) {
-    const int lane = threadIdx.x & 63, head = blockIdx.y, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.n_q) return;
-    int b = -1, q0 = 0, q1 = 0;
-    if (decode) b = row, q0 = row, q1 = row + 1;
-    else
-        for (int s = 0; s < a.n_seq; ++s) {
-            seq_rows(a.cu_q, s, a.n_q, &q0, &q1);
-            if (row >= q0 && row < q1) { b = s; break; }
-        }
-    if (b < 0) return;
-    int k0 = 0, lk;
-    if (PAGED) lk = (int)min((int64_t)max(a.kv_len[b], 0), (int64_t)a.n_table << a.page_shift);
-    else {
-        int k1;
-        seq_rows(a.cu_kv, b, a.n_kv, &k0, &k1);
-        lk = k1 - k0;
-    }
-    const int seen = min(lk, lk - (q1 - q0) + (row - q0) + 1);
-    const int D = a.head_dim, hk = head / a.group;
-    const T *q = (const T *)a.q + row * a.q_ld + head * a.q_hs;
-    float m = -INFINITY, l = 0, o0 = 0, o1 = 0;
-    for (int j0 = 0; j0 < seen; j0 += 64) {
-        const int j = j0 + lane;
-        int64_t ko = 0, vo = 0;
-        bool in = j < seen;
-        if (PAGED) {
-            const int pg = in ? a.table[(int64_t)b * a.table_ld + (j >> a.page_shift)] : -1;
-            in = in && pg >= 0 && pg < a.n_pages;
-            ko = vo = (in ? pg : 0) * a.page_stride + (j & ((1 << a.page_shift) - 1)) * a.k_ld;
-        } else ko = (in ? k0 + j : 0) * a.k_ld, vo = (in ? k0 + j : 0) * a.v_ld;
-        float s = -INFINITY;
-        if (in) {
-            const T *k = (const T *)a.k + ko + hk * a.k_hs;
-            s = 0;
-            for (int d = 0; d < D; ++d) s = fmaf((float)q[d], (float)k[d], s);
-            s *= a.scale_log2;
-        }
-        float mx = s;
-        for (int o = 32; o; o >>= 1) mx = fmaxf(mx, __shfl_xor(mx, o));
-        const float mn = fmaxf(m, mx), ref = mn == -INFINITY ? 0.f : mn;
-        const float c = exp2f(m - ref), p = exp2f(s - ref);
-        float ps = p;
-        for (int o = 32; o; o >>= 1) ps += __shfl_xor(ps, o);
-        l = l * c + ps, o0 *= c, o1 *= c, m = mn;
-        const unsigned long long live = __ballot(in);
-        for (int t = 0; t < 64; ++t) {
-            if (!(live >> t & 1)) continue;
-            const float pt = __shfl(p, t);
-            const T *v = (const T *)a.v + __shfl(vo, t) + hk * a.v_hs;
-            if (lane < D) o0 = fmaf(pt, (float)v[lane], o0);
-            if (lane + 64 < D) o1 = fmaf(pt, (float)v[lane + 64], o1);
+// Keys of a chunk.  The host knows the page table's width, not the lengths.  512 keep a workgroup's life short (a wave has four tiles) beside
+// what starting and joining it costs; few sequences are cut finer until two workgroups for each CU have work, many long ones coarser to bound
+// the workspace.
+constexpr int DEC_WAVES = 4;
+static int decode_chunk(int64_t blocks, int64_t max_len) {
+    int64_t chunk = 512;
+    if (blocks * ((max_len + 511) / 512) < 512) chunk = 256;
+    while (blocks * ((max_len + chunk - 1) / chunk) > 16384 && chunk < max_len) chunk *= 2;
+    return (int)chunk;
+}
+static int64_t decode_blocks(int n_seq, int n_head, int n_head_kv) { return (int64_t)n_seq * n_head_kv * ((n_head / n_head_kv + 15) / 16); }
+
+// The workspace: for each (sequence, head, chunk) its output's D sums, then its maximum and sum.
+size_t attn_decode_workspace(int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_len) {
+    const int chunk = decode_chunk(decode_blocks(n_seq, n_head, n_head_kv), max_len);
+    const int64_t splits = (max_len + chunk - 1) / chunk;
+    return splits > 1 ? (size_t)n_seq * n_head * splits * (head_dim + 2) * 4 : 0;
+}
+
+__device__ inline int decode_len(const AttnArgs &a, int b) { return (int)min((int64_t)max(a.kv_len[b], 0), (int64_t)a.n_table << a.page_shift); }
+
+template <typename T, int DP>
+__global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, int chunk, int splits, int q_blocks) {
+    constexpr int KB = sizeof(T) == 2 ? 2 : 1, KT = 16 * KB, UNIT = 16 / sizeof(T), DS = DP / 32, DB = DP / 16;   // KB blocks of 16 keys make a tile
+    constexpr int CPR = DP / UNIT, RPP = 64 / CPR, PASSES = KT / RPP, VLD = DP + (sizeof(T) == 2 ? 16 : 4);
+    typedef typename Vec<T>::x8 x8;
+    typedef T xp __attribute__((ext_vector_type(4 * KB)));             // a lane's part of P and V^T
+    __shared__ __attribute__((aligned(16))) T vs[DEC_WAVES][KT * VLD];
+    __shared__ float ms[DEC_WAVES][16], ls[DEC_WAVES][16];
+    static_assert(RPP <= 16 && 16 % RPP == 0, "a pass of V stays inside a block of 16 keys");
+    static_assert(KT * VLD * sizeof(T) >= 16 * DP * 4, "a wave's outputs fit where its V was");
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n = lane & 15, g = lane >> 4;
+    const int n_head_kv = a.n_head / a.group;
+    int x = blockIdx.x;
+    const int qb = x % q_blocks;
+    x /= q_blocks;
+    const int hk = x % n_head_kv;
+    x /= n_head_kv;
+    const int b = x % a.n_seq, split = x / a.n_seq;
+    const int len = decode_len(a, b), c0 = split * chunk, c1 = min(c0 + chunk, len);
+    if (c0 >= len && split) return;
+    const int D = a.head_dim, heads = min(16, a.group - 16 * qb), head0 = hk * a.group + 16 * qb;
+
+    x8 qf[DS];
+    {
+        const T *q = (const T *)a.q + b * a.q_ld + (head0 + (n < heads ? n : 0)) * a.q_hs;
+#pragma unroll
+        for (int s = 0; s < DS; ++s) {
+            const int d = 32 * s + 8 * g;
+            qf[s] = n < heads && d < D ? *(const x8 *)(q + d) : (x8)(T)0;
         }
     }
-    T *o = (T *)a.out + row * a.o_ld + head * a.o_hs;
-    const float r = l > 0 || l != l ? 1 / l : 0.f;
-    if (lane < D) o[lane] = (T)(o0 * r);
-    if (lane + 64 < D) o[lane + 64] = (T)(o1 * r);
+    const int tiles = (c1 - c0 + KT - 1) / KT;                         // this wave: tiles wave, wave + 4, ...
+    const int32_t *table = a.table + (int64_t)b * a.table_ld;
+    const int smask = (1 << a.page_shift) - 1;
+    const int vc = (lane % CPR) * UNIT, vrow = lane / CPR;
+    const T *kbase = (const T *)a.k + hk * a.k_hs, *vbase = (const T *)a.v + hk * a.v_hs + vc;
+
+    // Page numbers of the wave's next 64 blocks of 16 keys, one a lane; -1: no page there.
+    int pages = 0, batch = -1;
+    auto page_of = [&](int i, int kb) {                                // block kb of the wave's i-th tile
+        const int at = i * KB + kb;
+        if (at >> 6 != batch) {
+            batch = at >> 6;
+            const int e = batch * 64 + lane, j = c0 + ((e / KB) * DEC_WAVES + wave) * KT + (e % KB) * 16;
+            const int p = j < c1 ? table[j >> a.page_shift] : -1;
+            pages = p >= 0 && p < a.n_pages ? p : -1;
+        }
+        return __builtin_amdgcn_readlane(pages, at & 63);
+    };
+    x8 kr[KB][DS];
+    u32x4 vr[PASSES];
+    uint32_t there = 0, there_next = 0;
+    auto load_k = [&](int i) {
+        const int kv = c0 + (i * DEC_WAVES + wave) * KT;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            const int p = page_of(i, kb), j = kv + 16 * kb + n;
+            const T *k = kbase + p * a.page_stride + (j & smask) * a.k_ld;
+            const bool in = p >= 0 && j < c1;
+#pragma unroll
+            for (int s = 0; s < DS; ++s) {
+                const int d = 32 * s + 8 * g;
+                kr[kb][s] = (x8)(T)0;
+                if (in && d < D) kr[kb][s] = *(const x8 *)(k + d);
+            }
+        }
+    };
+    auto load_v = [&](int i) {
+        const int kv = c0 + (i * DEC_WAVES + wave) * KT;
+        int p[KB];
+        there_next = 0;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) p[kb] = page_of(i, kb), there_next |= (p[kb] >= 0) << kb;
+#pragma unroll
+        for (int s = 0; s < PASSES; ++s) {
+            const int r = vrow + RPP * s, j = kv + r;
+            const int pg = p[(RPP * s) >> 4];                          // (a pass stays inside a block of 16)
+            vr[s] = (u32x4)0u;
+            if (pg >= 0 && j < c1 && vc < D) vr[s] = *(const u32x4 *)(vbase + pg * a.page_stride + (j & smask) * a.v_ld);
+        }
+    };
+
+    f32x4 o[DB];
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[d] = (f32x4)0.f;
+    float m = -INFINITY, l = 0;                                        // of column n; l: this lane's keys
+    T *v = vs[wave];
+    if (wave < tiles) load_k(0), load_v(0);
+    for (int i = 0; i * DEC_WAVES + wave < tiles; ++i) {
+        const int kv = c0 + (i * DEC_WAVES + wave) * KT;
+        const bool more = (i + 1) * DEC_WAVES + wave < tiles;
+        there = there_next;
+        f32x4 s[KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+            s[kb] = (f32x4)0.f;
+#pragma unroll
+            for (int st = 0; st < DS; ++st) s[kb] = mfma16(kr[kb][st], qf[st], s[kb]);
+        }
+        if (more) load_k(i + 1);
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) *(u32x4 *)(v + (vrow + RPP * p) * VLD + vc) = vr[p];
+        if (more) load_v(i + 1);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (kv + KT > c1 || there != (1u << KB) - 1)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s[kb][r] = kv + 16 * kb + 4 * g + r < c1 && (there >> kb & 1) ? s[kb][r] : -INFINITY;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) mx = fmaxf(mx, s[kb][r]);
+        mx *= a.scale_log2;
+        if (__any(mx > m + 8.f)) {                                     // (the reference may lag the maximum by 2^8: attn_prompt.hip)
+            mx = fmaxf(mx, __shfl_xor(mx, 16));
+            mx = fmaxf(mx, __shfl_xor(mx, 32));
+            const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn, l *= f;
+#pragma unroll
+            for (int d = 0; d < DB; ++d) o[d] *= f;
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+        xp p;
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.scale_log2, -ref));
+                l += e;
+                p[4 * kb + r] = (T)e;
+            }
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+            xp vt;                                                     // keys 4 g + 0..3 of each block at component 16 d + n
+            if constexpr (sizeof(T) == 2) {
+                const T *at = v + (4 * g + (n >> 2)) * VLD + 16 * d + 4 * (n & 3);
+                typedef short s16x8 __attribute__((ext_vector_type(8)));
+                const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(at + 16 * VLD));
+                vt = __builtin_bit_cast(xp, (s16x8)__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) vt[r] = v[(4 * g + r) * VLD + 16 * d + n];
+            }
+            o[d] = mfma16(vt, p, o[d]);
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+
+    // the four waves' parts
+    l += __shfl_xor(l, 16);
+    l += __shfl_xor(l, 32);
+    if (g == 0) ms[wave][n] = m, ls[wave][n] = l;
+    __syncthreads();
+    float M = ms[0][n];
+    for (int w = 1; w < DEC_WAVES; ++w) M = fmaxf(M, ms[w][n]);
+    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    float *mine = (float *)vs[wave];
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+        if (n < heads) *(f32x4 *)(mine + n * DP + 16 * d + 4 * g) = o[d] * f;
+    __syncthreads();
+    for (int e = threadIdx.x; e < heads * DP; e += 64 * DEC_WAVES) {
+        const int q = e / DP, d = e % DP;
+        if (d >= D) continue;
+        float mq = ms[0][q], lq = 0, sum = 0;
+        for (int w = 1; w < DEC_WAVES; ++w) mq = fmaxf(mq, ms[w][q]);
+        for (int w = 0; w < DEC_WAVES; ++w) {
+            lq += ms[w][q] == -INFINITY ? 0.f : ls[w][q] * __builtin_amdgcn_exp2f(ms[w][q] - mq);
+            sum += ((const float *)vs[w])[e];
+        }
+        const int head = head0 + q;
+        if (len <= chunk) {
+            ((T *)a.out)[b * a.o_ld + head * a.o_hs + d] = (T)(lq == 0 ? 0.f : sum / lq);
+        } else {
+            float *to = (float *)a.ws + (((int64_t)b * a.n_head + head) * splits + split) * (D + 2);
+            to[d] = sum;
+            if (d == 0) to[D] = mq, to[D + 1] = lq;
+        }
+    }
+}
+
+// The chunks of the sequences that have several: a workgroup for each (sequence, head), its two halves every other chunk.
+template <typename T>
+__global__ __launch_bounds__(256) void attn_join_k(AttnArgs a, int chunk, int splits) {
+    const int head = blockIdx.x % a.n_head, b = blockIdx.x / a.n_head, D = a.head_dim, d = threadIdx.x & 127, half = threadIdx.x >> 7;
+    const int len = decode_len(a, b);
+    if (len <= chunk) return;
+    const int n = (len + chunk - 1) / chunk;
+    const float *part = (const float *)a.ws + ((int64_t)b * a.n_head + head) * splits * (D + 2);
+    __shared__ float red[4], acc[128], den;
+    float M = -INFINITY;
+    for (int s = threadIdx.x; s < n; s += 256) M = fmaxf(M, part[(int64_t)s * (D + 2) + D]);
+    for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float sum = 0, l = 0;
+    for (int s = half; s < n; s += 2) {
+        const float *p = part + (int64_t)s * (D + 2);
+        const float f = p[D] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[D] - M);
+        l += p[D + 1] * f;
+        if (d < D && f != 0) sum += p[d] * f;
+    }
+    if (half) {
+        acc[d] = sum;
+        if (d == 0) den = l;
+    }
+    __syncthreads();
+    if (half == 0 && d < D) {
+        l += den;
+        ((T *)a.out)[b * a.o_ld + head * a.o_hs + d] = (T)(l == 0 ? 0.f : (sum + acc[d]) / l);
+    }
+}
+
+template <typename T>
+static hipError_t decode_launch(const AttnArgs &a, hipStream_t st) {
+    const int n_head_kv = a.n_head / a.group, q_blocks = (a.group + 15) / 16;
+    const int64_t max_len = (int64_t)a.n_table << a.page_shift, blocks = decode_blocks(a.n_seq, a.n_head, n_head_kv);
+    const int chunk = decode_chunk(blocks, max_len), splits = (int)((max_len + chunk - 1) / chunk);
+    if (blocks * splits > INT32_MAX || (int64_t)a.n_seq * a.n_head > INT32_MAX) return hipErrorInvalidValue;
+    const dim3 g((unsigned)(blocks * splits));
+    if (a.head_dim <= 32) attn_decode_k<T, 32><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);
+    else if (a.head_dim <= 64) attn_decode_k<T, 64><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);
+    else attn_decode_k<T, 128><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && splits > 1) {
+        attn_join_k<T><<<dim3((unsigned)(a.n_seq * a.n_head)), 256, 0, st>>>(a, chunk, splits);
+        e = hipGetLastError();
+    }
+    return e;
 }
 
 hipError_t attn_decode(const AttnArgs &a, int type, hipStream_t st) {
-    const dim3 g((a.n_q + 3) / 4, a.n_head);
     switch (type) {
-        case FL_TYPE_F32: attn_rows_k<float, true><<<g, 256, 0, st>>>(a, true); break;
-        case FL_TYPE_F16: attn_rows_k<h16, true><<<g, 256, 0, st>>>(a, true); break;
-        default: attn_rows_k<b16, true><<<g, 256, 0, st>>>(a, true); break;
+        case FL_TYPE_F32: return decode_launch<float>(a, st);
+        case FL_TYPE_F16: return decode_launch<h16>(a, st);
+        default: return decode_launch<b16>(a, st);
     }
-    return hipGetLastError();
 }
-size_t attn_decode_workspace(int, int, int, int, int64_t) { return 0; }
 
 }  // namespace fl

@@ -35,9 +35,8 @@ __device__ inline typename Vec<T>::x8 read_vt(const T *v, int row, int d0, int l
         // each group of 16 lanes reads 4 keys x 16 components, 4 components a lane, and gets them transposed
         const int L = lane & 15;
         const T *p = v + (row + 4 * h + (L >> 2)) * LD + d0 + ((lane >> 4) & 1) * 16 + 4 * (L & 3);
-        typedef __attribute__((address_space(3))) s16x4 *lds_p;
-        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p));
-        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_p)(p + 8 * LD));
+        const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p));
+        const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4)(p + 8 * LD));
         typedef short s16x8 __attribute__((ext_vector_type(8)));
         r = __builtin_bit_cast(typename Vec<T>::x8, (s16x8)__builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     } else {

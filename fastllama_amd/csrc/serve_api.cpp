@@ -1,7 +1,6 @@
 // serve_api.cpp -- C entry points of the serving operators (include/fastllama_hip.h): every argument that the host can see is checked here, the
 // rest (row starts, lengths, page numbers: device data) is cut to the buffers by the kernels.
 #include <hip/hip_runtime.h>
-#include <climits>
 #include <cmath>
 
 #include "../../include/fastllama_hip.h"
@@ -61,7 +60,7 @@ static int check_pages(const char *fn, const fl_kv_pages *c) {
 static int check_table(const char *fn, const fl_kv_pages *c, const int32_t *table, int table_ld, int n_table, int n_seq) {
     if (n_seq < 1 || n_table < 1 || table_ld < 0 || (n_seq > 1 && table_ld < n_table) || !table)
         return set_error(FL_EINVAL, "%s: page table of %d rows, %d pages each, row stride %d", fn, n_seq, n_table, table_ld);
-    if ((int64_t)n_table * c->page_size > INT_MAX - 1024) return set_error(FL_EINVAL, "%s: %d pages of %d: positions pass 31 bits", fn, n_table, c->page_size);
+    if ((int64_t)n_table * c->page_size > 1 << 30) return set_error(FL_EINVAL, "%s: %d pages of %d: more than 2^30 positions", fn, n_table, c->page_size);
     return FL_OK;
 }
 

@@ -37,6 +37,15 @@ __device__ inline f32x16 mfma32(Vec<float>::x8 a, Vec<float>::x8 b, f32x16 c) {
     return c;
 }
 
+__device__ inline f32x4 mfma16(Vec<h16>::x8 a, Vec<h16>::x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+__device__ inline f32x4 mfma16(Vec<b16>::x8 a, Vec<b16>::x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+template <int N>
+__device__ inline f32x4 mfma16(float __attribute__((ext_vector_type(N))) a, float __attribute__((ext_vector_type(N))) b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+}
+
 // The larger of a lane's value and that of the lane 32 away.
 __device__ inline float max_halves(float x) {
     const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
@@ -46,6 +55,8 @@ __device__ inline float sum_halves(float x) {
     const auto w = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
+
+typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
 
 template <typename T>
 __device__ inline bool finite(T x) { return fabsf((float)x) < INFINITY; }

@@ -163,7 +163,7 @@ int fl_mul_mat_q_f32(const fl_qtensor *W, const float *x_dev, int ldx, float *y_
  *
  * Sequences: row starts `cu` (n_seq + 1 of them, not falling), lengths, past positions and page numbers are DEVICE data, so a captured graph
  * may be replayed on new ones.  Values that leave the buffers are cut, not reported: rows to those that exist, lengths to the table's
- * n_table * page_size, and a page number outside 0..n_pages-1 stands for keys that are not there.  Rows outside every sequence are neither
+ * n_table * page_size (at most 2^30), and a page number outside 0..n_pages-1 stands for keys that are not there.  Rows outside every sequence are neither
  * read nor written.  Every entry point launches on `stream`, allocates nothing, waits for nothing and may be captured. */
 typedef struct {
     void *data_dev;                    /* element (row, head, d) at row * token_stride + head * head_stride + d */
