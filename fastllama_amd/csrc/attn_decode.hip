@@ -36,7 +36,7 @@ size_t attn_decode_workspace(int n_seq, int n_head, int n_head_kv, int head_dim,
     return splits > 1 ? (size_t)n_seq * n_head * splits * (head_dim + 2) * 4 : 0;
 }
 
-__device__ inline int decode_len(const AttnArgs &a, int b) { return (int)min((int64_t)max(a.kv_len[b], 0), (int64_t)a.n_table << a.page_shift); }
+__device__ inline int decode_len(const AttnArgs &a, int b) { return min(max(a.kv_len[b], 0), a.n_table << a.page_shift); }
 
 template <typename T, int DP>
 __global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, int chunk, int splits, int q_blocks) {
@@ -224,36 +224,37 @@ __global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, i
     }
 }
 
-// The chunks of the sequences that have several: a workgroup for each (sequence, head), its two halves every other chunk.
-template <typename T>
-__global__ __launch_bounds__(256) void attn_join_k(AttnArgs a, int chunk, int splits) {
-    const int head = blockIdx.x % a.n_head, b = blockIdx.x / a.n_head, D = a.head_dim, d = threadIdx.x & 127, half = threadIdx.x >> 7;
+// The chunks of the sequences that have several: a workgroup for each (sequence, head), GROUPS groups of 128 threads (one for each component) that
+// take every GROUPS-th chunk.
+template <typename T, int GROUPS>
+__global__ __launch_bounds__(128 * GROUPS) void attn_join_k(AttnArgs a, int chunk, int splits) {
+    const int head = blockIdx.x % a.n_head, b = blockIdx.x / a.n_head, D = a.head_dim, d = threadIdx.x & 127, g = threadIdx.x >> 7;
     const int len = decode_len(a, b);
     if (len <= chunk) return;
     const int n = (len + chunk - 1) / chunk;
     const float *part = (const float *)a.ws + ((int64_t)b * a.n_head + head) * splits * (D + 2);
-    __shared__ float red[4], acc[128], den;
+    __shared__ float red[2 * GROUPS], acc[GROUPS][128], den[GROUPS];
     float M = -INFINITY;
-    for (int s = threadIdx.x; s < n; s += 256) M = fmaxf(M, part[(int64_t)s * (D + 2) + D]);
+    for (int s = threadIdx.x; s < n; s += 128 * GROUPS) M = fmaxf(M, part[(int64_t)s * (D + 2) + D]);
     for (int o = 32; o; o >>= 1) M = fmaxf(M, __shfl_xor(M, o));
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = M;
     __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    for (int w = 0; w < 2 * GROUPS; ++w) M = fmaxf(M, red[w]);
     float sum = 0, l = 0;
-    for (int s = half; s < n; s += 2) {
+    const int dd = min(d, D - 1);
+#pragma unroll 4
+    for (int s = g; s < n; s += GROUPS) {
         const float *p = part + (int64_t)s * (D + 2);
-        const float f = p[D] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(p[D] - M);
-        l += p[D + 1] * f;
-        if (d < D && f != 0) sum += p[d] * f;
+        const float x = p[dd], m = p[D], ls = p[D + 1];
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+        l += f == 0 ? 0.f : ls * f, sum += f == 0 ? 0.f : x * f;
     }
-    if (half) {
-        acc[d] = sum;
-        if (d == 0) den = l;
-    }
+    acc[g][d] = sum;
+    if (d == 0) den[g] = l;
     __syncthreads();
-    if (half == 0 && d < D) {
-        l += den;
-        ((T *)a.out)[b * a.o_ld + head * a.o_hs + d] = (T)(l == 0 ? 0.f : (sum + acc[d]) / l);
+    if (g == 0 && d < D) {
+        for (int i = 1; i < GROUPS; ++i) l += den[i], sum += acc[i][d];
+        ((T *)a.out)[b * a.o_ld + head * a.o_hs + d] = (T)(l == 0 ? 0.f : sum / l);
     }
 }
 
@@ -269,7 +270,9 @@ static hipError_t decode_launch(const AttnArgs &a, hipStream_t st) {
     else attn_decode_k<T, 128><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && splits > 1) {
-        attn_join_k<T><<<dim3((unsigned)(a.n_seq * a.n_head)), 256, 0, st>>>(a, chunk, splits);
+        const dim3 j((unsigned)(a.n_seq * a.n_head));
+        if (splits <= 8) attn_join_k<T, 2><<<j, 256, 0, st>>>(a, chunk, splits);
+        else attn_join_k<T, 8><<<j, 1024, 0, st>>>(a, chunk, splits);
         e = hipGetLastError();
     }
     return e;

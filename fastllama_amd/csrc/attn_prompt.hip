@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
     }
     if (b < 0) return;
     int k0 = 0, lk;
-    if (PAGED) lk = (int)min((int64_t)max(a.kv_len[b], 0), (int64_t)a.n_table << a.page_shift);
+    if (PAGED) lk = (int)min(max(a.kv_len[b], 0), a.n_table << a.page_shift);
     else {
         int k1;
         seq_rows(a.cu_kv, b, a.n_kv, &k0, &k1);
@@ -109,48 +109,60 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
         }
     }
 
-    // this thread's part of a tile: chunk c of rows pr + RPP * p
+    // This thread's part of a tile: chunk c of rows pr + RPP * p.  Addresses are a base of the pass that the scalar unit keeps and an offset of the
+    // thread that never changes.
     const int c = (t % CPR) * UNIT, pr = t / CPR;
-    const T *kbase = (const T *)a.k + hk * a.k_hs + c, *vbase = (const T *)a.v + hk * a.v_hs + c;
+    const char *kbase = (const char *)a.k + hk * a.k_hs * (int64_t)sizeof(T), *vbase = (const char *)a.v + hk * a.v_hs * (int64_t)sizeof(T);
+    const uint32_t koff = (uint32_t)((PAGED && RPP > 16 ? pr & 15 : pr) * a.k_ld + c) * (uint32_t)sizeof(T);
+    const uint32_t voff = (uint32_t)((PAGED && RPP > 16 ? pr & 15 : pr) * a.v_ld + c) * (uint32_t)sizeof(T);
     const int32_t *table = PAGED ? a.table + (int64_t)b * a.table_ld : nullptr;
     const int smask = (1 << a.page_shift) - 1;
     u32x4 kr[PASSES], vr[PASSES];
-    int pg[PASSES];
     uint32_t there = ~0u, there_next = ~0u;       // pages: a bit for each 16 keys of the tile that have a page
-    auto pages = [&](int tile) {
-#pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            const int j = tile * KT + pr + RPP * p;
-            pg[p] = j < end ? table[j >> a.page_shift] : -1;
-        }
-    };
+    int pages = -1;                               // page numbers of 64 blocks of 16 keys, one a lane; -1: none there
+    constexpr int BLOCKS = KT / 16, BATCH = 64 / BLOCKS;
     auto load = [&](int tile) {
-        if (PAGED) {
-            const int j = tile * KT + 16 * (lane & 3);
-            const int p = j < end ? table[j >> a.page_shift] : 0;
-            there_next = (uint32_t)__ballot(lane < KT / 16 && p >= 0 && p < a.n_pages);
+        const bool full = D == DP && (tile + 1) * KT <= end;
+        if constexpr (PAGED) {
+            if (tile % BATCH == 0) {
+                const int j = (tile * BLOCKS + lane) * 16, p = j < end ? table[j >> a.page_shift] : -1;
+                pages = p >= 0 && p < a.n_pages ? p : -1;
+            }
+            there_next = (uint32_t)(__ballot(pages >= 0) >> (tile % BATCH * BLOCKS)) & ((1u << BLOCKS) - 1);
         }
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-            const int j = tile * KT + pr + RPP * p;
-            bool in = j < end && c < D;
-            int64_t ko, vo;
-            if (PAGED) {
-                in = in && pg[p] >= 0 && pg[p] < a.n_pages;
-                ko = vo = (int64_t)pg[p] * a.page_stride + (j & smask) * a.k_ld;
-            } else ko = (int64_t)(k0 + j) * a.k_ld, vo = (int64_t)(k0 + j) * a.v_ld;
-            kr[p] = vr[p] = (u32x4)0u;
-            if (in) kr[p] = *(const u32x4 *)(kbase + ko), vr[p] = *(const u32x4 *)(vbase + vo);
+            const int j0 = tile * KT + RPP * p;                       // the pass's first key
+            const char *kp, *vp;
+            bool in = full || (j0 + pr < end && c < D);
+            if constexpr (!PAGED) {
+                kp = kbase + (k0 + j0) * a.k_ld * (int64_t)sizeof(T), vp = vbase + (k0 + j0) * a.v_ld * (int64_t)sizeof(T);
+            } else if constexpr (RPP <= 16) {                         // inside one block of 16 keys
+                const int pg = __builtin_amdgcn_readlane(pages, tile % BATCH * BLOCKS + RPP * p / 16);
+                const int64_t at = (pg * a.page_stride + (j0 & smask) * a.k_ld) * (int64_t)sizeof(T);
+                kp = kbase + at, vp = vbase + at;
+                in = in && pg >= 0;
+            } else {
+                const int j = j0 + (pr & ~15), pg = __shfl(pages, tile % BATCH * BLOCKS + (RPP * p + pr) / 16);
+                const int64_t at = (pg * a.page_stride + (j & smask) * a.k_ld) * (int64_t)sizeof(T);
+                kp = kbase + at, vp = vbase + at;
+                in = in && pg >= 0;
+            }
+            if (full && (!PAGED || there_next == (1u << BLOCKS) - 1)) {
+                kr[p] = *(const u32x4 *)(kp + koff), vr[p] = *(const u32x4 *)(vp + voff);
+            } else {
+                kr[p] = vr[p] = (u32x4)0u;
+                if (in) kr[p] = *(const u32x4 *)(kp + koff), vr[p] = *(const u32x4 *)(vp + voff);
+            }
         }
-        if (PAGED) pages(tile + 1);
     };
     // A value that is not finite may not reach a row that does not see it, and 0 times it is not 0: in the tiles that some row of the workgroup sees
     // in part it is stored as 0, and put back at the end for the rows that do see it.
     const int whole = past + min(r0, rows - 1) / a.group + 1;      // every row sees the keys before this one
     auto store = [&](int buf, int tile) {
+        if ((tile + 1) * KT > whole) {
 #pragma unroll
-        for (int p = 0; p < PASSES; ++p) {
-            if ((tile + 1) * KT > whole) {
+            for (int p = 0; p < PASSES; ++p) {
                 typedef T xu __attribute__((ext_vector_type(UNIT)));
                 xu v = __builtin_bit_cast(xu, vr[p]);
                 bool any = false;
@@ -162,6 +174,9 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
                 if (any) odd = 1;
                 vr[p] = __builtin_bit_cast(u32x4, v);
             }
+        }
+#pragma unroll
+        for (int p = 0; p < PASSES; ++p) {
             *(u32x4 *)(ks[buf] + (pr + RPP * p) * KLD + c) = kr[p];
             *(u32x4 *)(vs[buf] + (pr + RPP * p) * VLD + c) = vr[p];
         }
@@ -170,8 +185,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
     f32x16 o[DB];
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = (f32x16)0.f;
-    float m = -INFINITY, l = 0;
-    if (PAGED) pages(0);
+    float m = -INFINITY, ls[4] = {0, 0, 0, 0};                        // the sum in four chains
     if (tiles) {
         load(0);
         store(0, 0);
@@ -206,7 +220,9 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
             mx = max_halves(mx) * a.scale_log2;
             if (__any(mx > m + 8.f)) {
                 const float mn = fmaxf(m, mx), f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                m = mn, l *= f;
+                m = mn;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) ls[i] *= f;
 #pragma unroll
                 for (int d = 0; d < DB; ++d) o[d] *= f;
             }
@@ -217,7 +233,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.scale_log2, -ref));
-                    l += e;
+                    ls[r & 3] += e;
                     p[kb][r >> 3][r & 7] = (T)e;
                 }
 #pragma unroll
@@ -230,7 +246,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
             there = there_next;
         }
     }
-    l = sum_halves(l);
+    const float l = sum_halves((ls[0] + ls[1]) + (ls[2] + ls[3]));
     if (!valid) return;
     const float inv = l == 0 ? 0.f : 1 / l;
     if (tiles && odd)

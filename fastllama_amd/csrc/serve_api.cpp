@@ -26,14 +26,15 @@ static int check_dim(const char *fn, int type, int head_dim, int n_head_kv) {
     return FL_OK;
 }
 
-// Rows are read and written in 16-byte pieces.
+// Rows are read and written in 16-byte pieces, and 64 of them are within 32 bits of an address.
+constexpr int64_t MAX_ROW = 1 << 22;
 static int check_heads(const char *fn, const char *what, const fl_heads *h, int type, int rows) {
     if (!h || rows < 0) return set_error(FL_EINVAL, "%s: %s: null view or %d rows", fn, what, rows);
     if (rows == 0) return FL_OK;
     if (!h->data_dev) return set_error(FL_EINVAL, "%s: %s: null data", fn, what);
     const int unit = 16 / size_of(type);
-    if (!aligned(h->data_dev, 16) || h->token_stride < 0 || h->head_stride < 0 || h->token_stride % unit || h->head_stride % unit)
-        return set_error(FL_EINVAL, "%s: %s: data or strides (%lld, %lld) not aligned to 16 bytes", fn, what, (long long)h->token_stride, (long long)h->head_stride);
+    if (!aligned(h->data_dev, 16) || h->token_stride < 0 || h->head_stride < 0 || h->token_stride > MAX_ROW || h->token_stride % unit || h->head_stride % unit)
+        return set_error(FL_EINVAL, "%s: %s: data or strides (%lld, %lld) not multiples of 16 bytes, or past 2^22 elements", fn, what, (long long)h->token_stride, (long long)h->head_stride);
     return FL_OK;
 }
 
@@ -51,9 +52,9 @@ static int check_pages(const char *fn, const fl_kv_pages *c) {
         return set_error(FL_EINVAL, "%s: page_size %d is not a power of two in 16..65536", fn, c->page_size);
     if (c->n_pages < 1 || !c->k_dev || !c->v_dev) return set_error(FL_EINVAL, "%s: a cache of %d pages, or null pages", fn, c->n_pages);
     const int unit = 16 / size_of(c->type);
-    if (!aligned(c->k_dev, 16) || !aligned(c->v_dev, 16) || c->page_stride < 0 || c->head_stride < 0 || c->slot_stride < 0 || c->page_stride % unit ||
+    if (!aligned(c->k_dev, 16) || !aligned(c->v_dev, 16) || c->page_stride < 0 || c->head_stride < 0 || c->slot_stride < 0 || c->slot_stride > MAX_ROW || c->page_stride % unit ||
         c->head_stride % unit || c->slot_stride % unit)
-        return set_error(FL_EINVAL, "%s: pages or their strides are not aligned to 16 bytes", fn);
+        return set_error(FL_EINVAL, "%s: pages or their strides are not multiples of 16 bytes, or slot_stride past 2^22", fn);
     return FL_OK;
 }
 
