@@ -1410,12 +1410,13 @@ int fl_model_logits_nll(fl_model *m, int row0, int rows, const int32_t *next_tok
 int fl_model_logits_sample(fl_model *m, int row0, int rows, const float *u_host, const fl_sample_params *p, int32_t *tokens_host) {
     if (!m || !m->finalized || !u_host || !p || !tokens_host || row0 < 0 || rows < 1 || rows > m->B - row0)
         return set_error(FL_EINVAL, "fl_model_logits_sample: bad argument");
-    float *u = nullptr;                                          // rows numbers, and the tokens behind them
-    M_HIP(hipMalloc((void **)&u, (size_t)rows * 8));
+    const size_t ws = fl_sample_workspace(rows, m->V), head = ((size_t)rows * 8 + 15) / 16 * 16;
+    float *u = nullptr;                                          // rows numbers, the tokens behind them, then the workspace
+    M_HIP(hipMalloc((void **)&u, head + ws));
     int32_t *out = reinterpret_cast<int32_t *>(u + rows);
     int rc = FL_OK;
     hipError_t e = hipMemcpyAsync(u, u_host, (size_t)rows * 4, hipMemcpyHostToDevice, m->stream);
-    if (e == hipSuccess) rc = fl_sample(FL_TYPE_F32, m->logits + (size_t)row0 * m->ldl, m->ldl, rows, m->V, u, p, out, m->stream);
+    if (e == hipSuccess) rc = fl_sample(FL_TYPE_F32, m->logits + (size_t)row0 * m->ldl, m->ldl, rows, m->V, u, p, out, reinterpret_cast<char *>(u) + head, ws, m->stream);
     if (e == hipSuccess && rc == FL_OK) e = hipMemcpyAsync(tokens_host, out, (size_t)rows * 4, hipMemcpyDeviceToHost, m->stream);
     const hipError_t f = hipStreamSynchronize(m->stream);        // (also behind a failure: u_host and u are the stream's until then)
     (void)hipFree(u);

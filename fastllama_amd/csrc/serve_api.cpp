@@ -147,7 +147,10 @@ int fl_attn_pages(const fl_kv_pages *c, int n_head, float scale, const fl_heads 
     return e == hipSuccess ? FL_OK : hip_fail(e, fn);
 }
 
-int fl_sample(int type, const void *logits_dev, int64_t ld, int rows, int n_vocab, const float *u_dev, const fl_sample_params *p, int32_t *tokens_dev, void *stream) {
+size_t fl_sample_workspace(int rows, int n_vocab) { return rows < 1 || n_vocab < 1 || n_vocab > FL_SAMPLE_MAX_VOCAB ? 0 : sample_workspace(rows, n_vocab); }
+
+int fl_sample(int type, const void *logits_dev, int64_t ld, int rows, int n_vocab, const float *u_dev, const fl_sample_params *p, int32_t *tokens_dev,
+              void *workspace_dev, size_t workspace_bytes, void *stream) {
     const char *fn = "fl_sample";
     if (!size_of(type)) return set_error(FL_EINVAL, "%s: type %d is not f32 (0), f16 (1) or bf16 (%d)", fn, type, FL_TYPE_BF16);
     if (rows < 0 || n_vocab < 1 || n_vocab > FL_SAMPLE_MAX_VOCAB || ld < 0 || (rows > 1 && ld < n_vocab))
@@ -155,9 +158,12 @@ int fl_sample(int type, const void *logits_dev, int64_t ld, int rows, int n_voca
     if (rows == 0) return FL_OK;
     if (!logits_dev || !u_dev || !p || !tokens_dev) return set_error(FL_EINVAL, "%s: null argument", fn);
     if (!aligned(logits_dev, (size_t)size_of(type))) return set_error(FL_EINVAL, "%s: logits not aligned to their type", fn);
+    const size_t need = sample_workspace(rows, n_vocab);
+    if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16))
+        return set_error(FL_EINVAL, "%s: a workspace of %zu bytes, aligned to 16 (want %zu: fl_sample_workspace)", fn, workspace_dev ? workspace_bytes : 0, need);
     FL_TRY(ensure_device());
     SampleArgs a{};
-    a.logits = logits_dev, a.ld = ld, a.rows = rows, a.n_vocab = n_vocab, a.u = u_dev, a.tokens = tokens_dev;
+    a.logits = logits_dev, a.ld = ld, a.rows = rows, a.n_vocab = n_vocab, a.u = u_dev, a.tokens = tokens_dev, a.ws = workspace_dev;
     a.temperature_p = p->temperature_dev, a.top_k_p = p->top_k_dev, a.top_p_p = p->top_p_dev, a.min_p_p = p->min_p_dev;
     a.temperature = p->temperature, a.top_k = p->top_k, a.top_p = p->top_p, a.min_p = p->min_p;
     const hipError_t e = sample(a, type, S(stream));

@@ -112,7 +112,9 @@ _PROTOS = {
     "fl_attn_pages_workspace": (C.c_size_t, [C.POINTER(KVPagesDesc), C.c_int, C.c_int, C.c_int]),
     "fl_attn_pages": (C.c_int, [C.POINTER(KVPagesDesc), C.c_int, C.c_float, C.POINTER(Heads), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                 C.c_int, C.c_int, C.POINTER(Heads), C.c_void_p, C.c_size_t, C.c_void_p]),
-    "fl_sample": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.POINTER(SampleParams), C.c_void_p, C.c_void_p]),
+    "fl_sample": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.POINTER(SampleParams), C.c_void_p,
+                            C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fl_sample_workspace": (C.c_size_t, [C.c_int, C.c_int]),
     "fl_model_logits_sample": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.POINTER(SampleParams), C.c_void_p]),
     "fl_comm_unique_id": (C.c_int, [C.c_void_p]),
     "fl_comm_create": (C.c_void_p, [C.c_void_p, C.c_int, C.c_int]),

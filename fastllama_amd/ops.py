@@ -354,6 +354,9 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
         p.top_k = max(0, min(int(top_k), vocab))
     if out is None:
         out = torch.empty(rows, dtype=torch.int32, device=logits.device)
-    check(hip.load().fl_sample(_type(logits, "logits"), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, per_row(u, "u", torch.float32),
-                               C.byref(p), per_row(out, "out", torch.int32), _stream()), "fl_sample")
+    lib = hip.load()
+    size = lib.fl_sample_workspace(rows, vocab)
+    ws = torch.empty(size, dtype=torch.uint8, device=logits.device)
+    check(lib.fl_sample(_type(logits, "logits"), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, per_row(u, "u", torch.float32),
+                               C.byref(p), per_row(out, "out", torch.int32), ws.data_ptr(), size, _stream()), "fl_sample")
     return out

@@ -199,7 +199,7 @@ int fl_attn_pages(const fl_kv_pages *c, int n_head, float scale, const fl_heads 
  * always.  The token is the first kept index, in rising order, at which the running sum of the kept w exceeds u times their sum, u in [0, 1).
  * temperature <= 0: the first index of the largest logit.  NaN counts as -infinity; a row of nothing else gives -1; logits of +infinity share the weight.
  * The w are held in 2^-44 units (a token below that never comes up), sums of them are exact.  A *_dev pointer gives each row its own setting, NULL
- * the scalar beside it to all. */
+ * the scalar beside it to all.  The workspace of fl_sample_workspace() bytes is no other call's at the same time. */
 #define FL_SAMPLE_MAX_VOCAB 262144
 typedef struct {
     const float *temperature_dev;
@@ -209,8 +209,9 @@ typedef struct {
     int top_k;
     float top_p, min_p;
 } fl_sample_params;
+size_t fl_sample_workspace(int rows, int n_vocab);
 int fl_sample(int type, const void *logits_dev, int64_t ld, int rows, int n_vocab, const float *u_dev, const fl_sample_params *p, int32_t *tokens_dev,
-              void *stream);
+              void *workspace_dev, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------- collectives (RCCL over xGMI) -- */
 /* New for SURVEY.md section 8(e): the reference is single-process.  One process per GPU; rank 0 creates

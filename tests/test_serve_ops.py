@@ -90,17 +90,21 @@ def test_pages_workspace(L):
     assert L.fl_attn_pages_workspace(None, 4, 5, 2) == 0 and L.fl_attn_pages_workspace(cache(), 0, 5, 2) == 0
 
 
-def sample(L, type=hip.F32, l=P, ld=100, rows=2, V=100, u=P, p=C.byref(hip.SampleParams()), out=P):
-    return L.fl_sample(type, l, ld, rows, V, u, p, out, None)
+def sample(L, type=hip.F32, l=P, ld=100, rows=2, V=100, u=P, p=C.byref(hip.SampleParams()), out=P, ws=P, size=1 << 40):
+    return L.fl_sample(type, l, ld, rows, V, u, p, out, ws, size, None)
 
 
 def test_sample_refuses(L):
     assert sample(L) == GOOD and sample(L, V=hip.SAMPLE_MAX_VOCAB, ld=hip.SAMPLE_MAX_VOCAB) == GOOD and sample(L, rows=1, ld=0) == GOOD
     for kw in (dict(type=2), dict(l=None), dict(l=P + 2), dict(ld=99), dict(ld=-1), dict(rows=-1), dict(V=0), dict(V=hip.SAMPLE_MAX_VOCAB + 1, ld=1 << 20), dict(u=None),
-               dict(p=None), dict(out=None)):
+               dict(p=None), dict(out=None), dict(ws=None), dict(ws=P + 8), dict(size=L.fl_sample_workspace(2, 100) - 1)):
         assert sample(L, **kw) == hip.FL_EINVAL, kw
         assert b"fl_sample" in L.fl_last_error()
     assert sample(L, rows=0, l=None) == hip.FL_OK
+    for rows, V in ((1, 1), (3, 4097), (200, 32000), (5000, 262144)):
+        size = L.fl_sample_workspace(rows, V)
+        assert size > 0 and sample(L, rows=rows, V=V, ld=V, size=size) == GOOD and sample(L, rows=rows, V=V, ld=V, size=size - 1) == hip.FL_EINVAL
+    assert L.fl_sample_workspace(0, 5) == 0 and L.fl_sample_workspace(5, 0) == 0 and L.fl_sample_workspace(5, 1 << 30) == 0
     assert L.fl_model_logits_sample(None, 0, 1, P, C.byref(hip.SampleParams()), P) == hip.FL_EINVAL
 
 
