@@ -48,9 +48,9 @@ struct Weigher {
     double max, c;
     const double *table;
     __device__ u64 of(float x) const {
-        if (x == top) return 1ull << S_BITS;                   // (also +infinity, which is no distance from itself)
-        const double y = ((double)x - max) * c;
-        if (!(y > -(S_BITS + 2))) return 0;
+        const double d = ((double)x - max) * c;
+        const bool some = d > -(S_BITS + 2);                          // (otherwise 0; no number where both are infinite)
+        const double y = some ? d : 0.0;
         constexpr double shift = 6755399441055744.0 / 32;             // 1.5 * 2^52 / 32: the sum's last bits are 32 y rounded
         const double r = y + shift, f = y - (r - shift);
         const int k = (int)(uint32_t)__double_as_longlong(r);
@@ -62,7 +62,8 @@ struct Weigher {
         p = fma(p, f, 1.0);
         const double t = __longlong_as_double(__double_as_longlong(table[k & 31]) + ((long long)(k >> 5) << 52));
         const double w = fma(t, p, 4503599627370496.0);               // + 2^52: the fraction's bits are the rounded whole number
-        return (u64)__double_as_longlong(w) & ((1ull << 52) - 1);
+        const u64 v = some ? (u64)__double_as_longlong(w) & ((1ull << 52) - 1) : 0;
+        return x == top ? 1ull << S_BITS : v;                         // (also +infinity, which is no distance from itself)
     }
     __device__ u64 of_key(uint32_t key) const { return key ? of(value_of(key)) : 0; }
 };
@@ -462,11 +463,12 @@ __device__ void cut(Shared &s, const Src &src, u64 need, In in, uint32_t *tkey, 
             const u64 own = s.lw[t];
             u64 sum = 0;
             uint32_t same = 1;
-#pragma unroll 4
+#pragma unroll 8
             for (int j = 0; j < n; ++j) {
-                const uint32_t kj = s.lkey[j];
-                const bool tie = kj == key && s.lidx[j] < idx;
-                sum += kj > key || tie ? s.lw[j] : 0;
+                const uint32_t kj = s.lkey[j], ij = s.lidx[j];
+                const u64 wj = s.lw[j];
+                const bool tie = (kj == key) & (ij < idx);
+                sum += (kj > key) | tie ? wj : 0;
                 same += tie;
             }
             if (sum < need && sum + own >= need) s.prefix = key, s.need = same;
@@ -586,11 +588,11 @@ __device__ void pick(Shared &s, const Src &src, const Kept &k, float u, int32_t 
         const bool eq = tied && x == k.tkey;
         u64 w = x > k.tkey ? src.weight(i + lane, x) : 0;
         w = w >= k.wmin ? w : 0;
-        const uint32_t eq_incl = wave_scan((uint32_t)eq);
-        if (eq) w = seen + eq_incl - 1 < k.ties ? k.wt : 0;
+        const unsigned long long eqs = __ballot(eq);
+        if (eq) w = seen + __popcll(eqs & ((1ull << lane) - 1)) < k.ties ? k.wt : 0;
         const u64 incl = wave_scan(w), pos = run + incl - w;
         if (pos <= target && target < pos + w) *token = src.index(i + lane);
-        run += __shfl(incl, 63), seen += __shfl(eq_incl, 63);
+        run += __shfl(incl, 63), seen += __popcll(eqs);
         if (target < run) return;
     }
 }
@@ -606,9 +608,10 @@ __device__ inline void draw_short(Shared &s, int n, int top_k, float top_p, u64 
         idx = s.lidx[t], w = s.lw[t];
 #pragma unroll 8
         for (int j = 0; j < n; ++j) {
-            const uint32_t kj = s.lkey[j];
-            const bool before = kj > key || (kj == key && s.lidx[j] < idx);
-            rank += before, sum += before ? s.lw[j] : 0;
+            const uint32_t kj = s.lkey[j], ij = s.lidx[j];
+            const u64 wj = s.lw[j];
+            const bool before = (kj > key) | ((kj == key) & (ij < idx));
+            rank += before, sum += before ? wj : 0;
         }
         if (rank == top_k - 1) s.need = sum + w;                       // the sum of the first top_k
     }
@@ -622,7 +625,8 @@ __device__ inline void draw_short(Shared &s, int n, int top_k, float top_p, u64 
 #pragma unroll 8
     for (int j = 0; j < n; ++j) {
         const u64 x = s.lw[j];
-        total += x, run += s.lidx[j] < idx ? x : 0;
+        const uint32_t ij = s.lidx[j];
+        total += x, run += ij < idx ? x : 0;
     }
     const u64 target = target_of(u, total);
     if (run <= target && target < run + kept) *token = (int32_t)idx;
@@ -676,13 +680,17 @@ __global__ __launch_bounds__(S_THREADS) void sample_draw_k(SampleArgs a, PowerTa
     // The parts' sums are known but for what of the lists is kept: the part that holds the target, then the token in it.
     auto pick_part = [&]() {
         const bool tied = k.tkey && k.wt >= k.wmin;
-        u64 sum = lane < parts ? w.part[lane].sum : 0;
-        uint32_t eq = 0;
-        for (int i = past - held; i < past; ++i) {
+        if (t < 64) s.lw[t] = t < parts ? w.part[t].sum : 0, s.lidx[t] = 0;
+        __syncthreads();
+        for (int i = t; cuts && i < n; i += S_THREADS) {
+            const uint32_t key = s.key[i], at = s.idx[i] / (uint32_t)part_len;
             const u64 x = s.weight[i];
-            if (s.key[i] > k.tkey) sum += x >= k.wmin ? x : 0;
-            else eq += tied && s.key[i] == k.tkey;
+            if (key > k.tkey && x >= k.wmin) atomicAdd(&s.lw[at], x);
+            if (tied && key == k.tkey) atomicAdd(&s.lidx[at], 1u);
         }
+        __syncthreads();
+        const u64 sum = s.lw[lane];
+        const uint32_t eq = s.lidx[lane];
         const u64 sums = wave_scan(sum), before = sums - sum;
         const uint32_t eqs = wave_scan(eq);
         const u64 run = before + min((u64)(eqs - eq), k.ties) * k.wt, end = sums + min((u64)eqs, k.ties) * k.wt;
