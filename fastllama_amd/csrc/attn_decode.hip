@@ -17,21 +17,24 @@
 
 namespace fl {
 
-// Keys of a chunk.  The host knows the page table's width, not the lengths.  512 keep a workgroup's life short (a wave has four tiles) beside
-// what starting and joining it costs; few sequences are cut finer until two workgroups for each CU have work, many long ones coarser to bound
-// the workspace.
+// Keys of a chunk.  The host knows the page table's width, not the lengths.  512 keep a workgroup's life short (a wave has four tiles of f16) beside
+// what starting and joining it costs: 16 sequences of 2048, 32 heads of 128 in f16 take 117 us at 128, 106 at 256, 105 at 512, 103 at 1024; 64 of 1 to
+// 4096, 8 key heads, 48, 39, 35, 38.  Few sequences are cut finer until each CU could have two workgroups, down to a tile a wave: one of 300, 32 heads
+// in f32, takes 14.3 us at 512 and 9.7 at 64.  Many long ones are cut coarser to bound the workspace.
 constexpr int DEC_WAVES = 4;
-static int decode_chunk(int64_t blocks, int64_t max_len) {
+static int decode_chunk(int64_t blocks, int64_t max_len, int least) {
     int64_t chunk = 512;
-    if (blocks * ((max_len + 511) / 512) < 512) chunk = 256;
+    if (max_len <= 2 * least) return 512;              // (two tiles a wave: 7.3 us for 256 keys in f16, 8.9 cut in two and joined)
+    while (chunk > least && blocks * ((max_len + chunk - 1) / chunk) < 512) chunk /= 2;
     while (blocks * ((max_len + chunk - 1) / chunk) > 16384 && chunk < max_len) chunk *= 2;
     return (int)chunk;
 }
+static int least_chunk(int type) { return type == FL_TYPE_F32 ? 16 * DEC_WAVES : 32 * DEC_WAVES; }
 static int64_t decode_blocks(int n_seq, int n_head, int n_head_kv) { return (int64_t)n_seq * n_head_kv * ((n_head / n_head_kv + 15) / 16); }
 
 // The workspace: for each (sequence, head, chunk) its output's D sums, then its maximum and sum.
-size_t attn_decode_workspace(int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_len) {
-    const int chunk = decode_chunk(decode_blocks(n_seq, n_head, n_head_kv), max_len);
+size_t attn_decode_workspace(int type, int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_len) {
+    const int chunk = decode_chunk(decode_blocks(n_seq, n_head, n_head_kv), max_len, least_chunk(type));
     const int64_t splits = (max_len + chunk - 1) / chunk;
     return splits > 1 ? (size_t)n_seq * n_head * splits * (head_dim + 2) * 4 : 0;
 }
@@ -262,7 +265,7 @@ template <typename T>
 static hipError_t decode_launch(const AttnArgs &a, hipStream_t st) {
     const int n_head_kv = a.n_head / a.group, q_blocks = (a.group + 15) / 16;
     const int64_t max_len = (int64_t)a.n_table << a.page_shift, blocks = decode_blocks(a.n_seq, a.n_head, n_head_kv);
-    const int chunk = decode_chunk(blocks, max_len), splits = (int)((max_len + chunk - 1) / chunk);
+    const int chunk = decode_chunk(blocks, max_len, sizeof(T) == 4 ? 16 * DEC_WAVES : 32 * DEC_WAVES), splits = (int)((max_len + chunk - 1) / chunk);
     if (blocks * splits > INT32_MAX || (int64_t)a.n_seq * a.n_head > INT32_MAX) return hipErrorInvalidValue;
     const dim3 g((unsigned)(blocks * splits));
     if (a.head_dim <= 32) attn_decode_k<T, 32><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);

@@ -19,7 +19,6 @@
 
 namespace fl {
 
-constexpr int PR_ROWS = 128;             // rows of a workgroup: 4 waves of 32
 
 template <typename T>
 struct Tile {                            // LDS tiles of a type
@@ -47,12 +46,13 @@ __device__ inline typename Vec<T>::x8 read_vt(const T *v, int row, int d0, int l
     return r;
 }
 
-template <typename T, int DP, bool PAGED>
+// KS: waves that share 32 rows, each with its part of every tile's keys; they join at the end.
+template <typename T, int DP, bool PAGED, int KS>
 __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int KT = Tile<T>::KT, KLD = DP + Tile<T>::KPAD, VLD = DP + Tile<T>::VPAD;
     constexpr int UNIT = 16 / sizeof(T), CPR = DP / UNIT, RPP = 256 / CPR, PASSES = KT / RPP;   // 16-byte chunks of a row, rows of a pass over the tile
-    constexpr int KB = KT / 32, DB = DP / 32, DS = DP / 16;
+    constexpr int KB = KT / 32 / KS, DB = DP / 32, DS = DP / 16, RW = 4 / KS, PR_ROWS = 32 * RW;   // KB blocks of 32 keys a wave, RW waves of rows
     static_assert(KT % RPP == 0 && PASSES >= 1, "a tile is whole passes of the workgroup");
     __shared__ __attribute__((aligned(16))) T ks[2][KT * KLD], vs[2][KT * VLD];
 
@@ -60,29 +60,57 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
     if (threadIdx.x == 0) odd = 0;
     __syncthreads();
 
-    const int t = threadIdx.x, lane = t & 63, h = lane >> 5, n_head_kv = a.n_head / a.group;
-    // workgroups go round the 8 XCDs by their number: with 8 key heads (or a multiple) all that read a head's keys share an L2; the blocks with most keys first
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, kb0 = wave / RW * KB, n_head_kv = a.n_head / a.group;
+    // Workgroups go round the 8 XCDs by their number: with 8 key heads (or a multiple) all that read a head's keys share an L2.
     const int hk = blockIdx.x % n_head_kv;
-    int blk = gridDim.x / n_head_kv - 1 - blockIdx.x / n_head_kv;
-
-    // the sequence that has block `blk` of all sequences' blocks: every wave scans 64 sequences at a time
-    int b = -1, q0 = 0, lq = 0;
-    for (int s0 = 0; s0 < a.n_seq; s0 += 64) {
-        int f = 0, e = 0;
-        if (s0 + lane < a.n_seq) seq_rows(a.cu_q, s0 + lane, a.n_q, &f, &e);
-        const int n = (int)(((int64_t)(e - f) * a.group + PR_ROWS - 1) / PR_ROWS);
-        int incl = n;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int up = __shfl_up(incl, o);
-            if (lane >= o) incl += up;
+    int blk = blockIdx.x / n_head_kv, b = -1, q0 = 0, lq = 0;
+    auto blocks_of = [&](int s, int *f, int *e) {                      // sequence s's first row and end; returns its blocks
+        *f = *e = 0;
+        if (s < a.n_seq) seq_rows(a.cu_q, s, a.n_q, f, e);
+        return (int)(((int64_t)(*e - *f) * a.group + PR_ROWS - 1) / PR_ROWS);
+    };
+    if (a.n_seq <= 64) {
+        // The longest ways first, or the last to start ends long behind the others: a block's number in its sequence is (but for keys of the past) its
+        // number of tiles, so the blocks go by that number, falling, through all sequences that have one of it.
+        int f, e;
+        const int n = blocks_of(lane, &f, &e);
+        auto most = [](int x) {
+            for (int o = 32; o; o >>= 1) x = max(x, __shfl_xor(x, o));
+            return __builtin_amdgcn_readfirstlane(x);
+        };
+        const int max1 = most(n), first = max1 ? __builtin_ctzll(__ballot(n == max1)) : 0, max2 = most(lane == first ? 0 : n);
+        int level = max1 - 1 - blk;                                    // (alone above the second longest)
+        if (level >= max2) blk = 0;
+        else {
+            blk -= max1 - max2, level = max2 - 1;
+            for (; level >= 0; --level) {
+                const int c = __popcll(__ballot(n > level));
+                if (blk < c) break;
+                blk -= c;
+            }
         }
-        const int total = __shfl(incl, 63);
-        if (blk < total) {
-            const int w = __ffsll((unsigned long long)__ballot(incl > blk)) - 1;
-            b = s0 + w, q0 = __shfl(f, w), lq = __shfl(e, w) - q0, blk -= __shfl(incl - n, w);
-            break;
+        if (level < 0) return;
+        const unsigned long long has = __ballot(n > level);
+        const int w = __builtin_ctzll(__ballot(n > level && __popcll(has & ((1ull << lane) - 1)) == blk));
+        b = w, q0 = __builtin_amdgcn_readlane(f, w), lq = __builtin_amdgcn_readlane(e, w) - q0, blk = level;
+    } else {
+        blk = gridDim.x / n_head_kv - 1 - blk;
+        for (int s0 = 0; s0 < a.n_seq; s0 += 64) {                     // 64 sequences at a time
+            int f, e;
+            const int n = blocks_of(s0 + lane, &f, &e);
+            int incl = n;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int up = __shfl_up(incl, o);
+                if (lane >= o) incl += up;
+            }
+            const int total = __builtin_amdgcn_readlane(incl, 63);
+            if (blk < total) {
+                const int w = __builtin_ctzll(__ballot(incl > blk));
+                b = s0 + w, q0 = __builtin_amdgcn_readlane(f, w), lq = __builtin_amdgcn_readlane(e, w) - q0, blk -= __builtin_amdgcn_readlane(incl - n, w);
+                break;
+            }
+            blk -= total;
         }
-        blk -= total;
     }
     if (b < 0) return;
     int k0 = 0, lk;
@@ -92,7 +120,7 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
         seq_rows(a.cu_kv, b, a.n_kv, &k0, &k1);
         lk = k1 - k0;
     }
-    const int D = a.head_dim, rows = lq * a.group, r0 = blk * PR_ROWS, rw = r0 + (t >> 6) * 32, row = rw + (lane & 31);
+    const int D = a.head_dim, rows = lq * a.group, r0 = blk * PR_ROWS, rw = r0 + wave % RW * 32, row = rw + (lane & 31);
     const bool valid = row < rows;
     const int tok = (valid ? row : rows - 1) / a.group, head = hk * a.group + (valid ? row : rows - 1) % a.group;
     const int past = lk - lq, lim = past + tok;                    // the last key that this lane's row sees
@@ -117,54 +145,62 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
     const uint32_t voff = (uint32_t)((PAGED && RPP > 16 ? pr & 15 : pr) * a.v_ld + c) * (uint32_t)sizeof(T);
     const int32_t *table = PAGED ? a.table + (int64_t)b * a.table_ld : nullptr;
     const int smask = (1 << a.page_shift) - 1;
-    u32x4 kr[PASSES], vr[PASSES];
-    uint32_t there = ~0u, there_next = ~0u;       // pages: a bit for each 16 keys of the tile that have a page
+    // A tile on its way to LDS; pages: a bit for each 16 keys that have a page.
+    struct Stage {
+        u32x4 k[PASSES], v[PASSES];
+        uint32_t there;
+    } stage;
     int pages = -1;                               // page numbers of 64 blocks of 16 keys, one a lane; -1: none there
     constexpr int BLOCKS = KT / 16, BATCH = 64 / BLOCKS;
-    auto load = [&](int tile) {
-        const bool full = D == DP && (tile + 1) * KT <= end;
+    constexpr uint32_t ALL = (1u << BLOCKS) - 1;
+    auto load = [&](int tile, Stage &to) {
+        to.there = ALL;
         if constexpr (PAGED) {
             if (tile % BATCH == 0) {
                 const int j = (tile * BLOCKS + lane) * 16, p = j < end ? table[j >> a.page_shift] : -1;
                 pages = p >= 0 && p < a.n_pages ? p : -1;
             }
-            there_next = (uint32_t)(__ballot(pages >= 0) >> (tile % BATCH * BLOCKS)) & ((1u << BLOCKS) - 1);
+            to.there = (uint32_t)(__ballot(pages >= 0) >> (tile % BATCH * BLOCKS)) & ALL;
         }
+        const char *kp[PASSES], *vp[PASSES];
+        bool page[PASSES];                                            // (of the pass's keys that this thread loads)
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
             const int j0 = tile * KT + RPP * p;                       // the pass's first key
-            const char *kp, *vp;
-            bool in = full || (j0 + pr < end && c < D);
+            page[p] = true;
             if constexpr (!PAGED) {
-                kp = kbase + (k0 + j0) * a.k_ld * (int64_t)sizeof(T), vp = vbase + (k0 + j0) * a.v_ld * (int64_t)sizeof(T);
-            } else if constexpr (RPP <= 16) {                         // inside one block of 16 keys
-                const int pg = __builtin_amdgcn_readlane(pages, tile % BATCH * BLOCKS + RPP * p / 16);
-                const int64_t at = (pg * a.page_stride + (j0 & smask) * a.k_ld) * (int64_t)sizeof(T);
-                kp = kbase + at, vp = vbase + at;
-                in = in && pg >= 0;
+                kp[p] = p ? kp[p - 1] + RPP * a.k_ld * (int64_t)sizeof(T) : kbase + (k0 + j0) * a.k_ld * (int64_t)sizeof(T);
+                vp[p] = p ? vp[p - 1] + RPP * a.v_ld * (int64_t)sizeof(T) : vbase + (k0 + j0) * a.v_ld * (int64_t)sizeof(T);
             } else {
-                const int j = j0 + (pr & ~15), pg = __shfl(pages, tile % BATCH * BLOCKS + (RPP * p + pr) / 16);
-                const int64_t at = (pg * a.page_stride + (j & smask) * a.k_ld) * (int64_t)sizeof(T);
-                kp = kbase + at, vp = vbase + at;
-                in = in && pg >= 0;
+                constexpr bool one = RPP <= 16;                       // a pass inside one block of 16 keys
+                const int j = one ? j0 : j0 + (pr & ~15), at = tile % BATCH * BLOCKS + (one ? RPP * p : RPP * p + pr) / 16;
+                const int pg = one ? __builtin_amdgcn_readlane(pages, at) : __shfl(pages, at);
+                const int64_t off = (pg * a.page_stride + (j & smask) * a.k_ld) * (int64_t)sizeof(T);
+                kp[p] = kbase + off, vp[p] = vbase + off;
+                page[p] = pg >= 0;
             }
-            if (full && (!PAGED || there_next == (1u << BLOCKS) - 1)) {
-                kr[p] = *(const u32x4 *)(kp + koff), vr[p] = *(const u32x4 *)(vp + voff);
-            } else {
-                kr[p] = vr[p] = (u32x4)0u;
-                if (in) kr[p] = *(const u32x4 *)(kp + koff), vr[p] = *(const u32x4 *)(vp + voff);
+            if constexpr (!PAGED || RPP <= 16) asm("" : "+s"(kp[p]), "+s"(vp[p]));   // (kept scalar: a load adds the thread's offset by itself)
+        }
+        if (D == DP && (tile + 1) * KT <= end && to.there == ALL) {
+#pragma unroll
+            for (int p = 0; p < PASSES; ++p) to.k[p] = *(const u32x4 *)(kp[p] + koff), to.v[p] = *(const u32x4 *)(vp[p] + voff);
+        } else {
+#pragma unroll
+            for (int p = 0; p < PASSES; ++p) {
+                to.k[p] = to.v[p] = (u32x4)0u;
+                if (tile * KT + RPP * p + pr < end && c < D && page[p]) to.k[p] = *(const u32x4 *)(kp[p] + koff), to.v[p] = *(const u32x4 *)(vp[p] + voff);
             }
         }
     };
     // A value that is not finite may not reach a row that does not see it, and 0 times it is not 0: in the tiles that some row of the workgroup sees
     // in part it is stored as 0, and put back at the end for the rows that do see it.
     const int whole = past + min(r0, rows - 1) / a.group + 1;      // every row sees the keys before this one
-    auto store = [&](int buf, int tile) {
+    auto store = [&](int buf, int tile, Stage &from) {
         if ((tile + 1) * KT > whole) {
 #pragma unroll
             for (int p = 0; p < PASSES; ++p) {
                 typedef T xu __attribute__((ext_vector_type(UNIT)));
-                xu v = __builtin_bit_cast(xu, vr[p]);
+                xu v = __builtin_bit_cast(xu, from.v[p]);
                 bool any = false;
 #pragma unroll
                 for (int e = 0; e < UNIT; ++e) {
@@ -172,13 +208,13 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
                     v[e] = finite(v[e]) ? v[e] : (T)0.f;
                 }
                 if (any) odd = 1;
-                vr[p] = __builtin_bit_cast(u32x4, v);
+                from.v[p] = __builtin_bit_cast(u32x4, v);
             }
         }
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-            *(u32x4 *)(ks[buf] + (pr + RPP * p) * KLD + c) = kr[p];
-            *(u32x4 *)(vs[buf] + (pr + RPP * p) * VLD + c) = vr[p];
+            *(u32x4 *)(ks[buf] + (pr + RPP * p) * KLD + c) = from.k[p];
+            *(u32x4 *)(vs[buf] + (pr + RPP * p) * VLD + c) = from.v[p];
         }
     };
 
@@ -186,26 +222,35 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
 #pragma unroll
     for (int d = 0; d < DB; ++d) o[d] = (f32x16)0.f;
     float m = -INFINITY, ls[4] = {0, 0, 0, 0};                        // the sum in four chains
-    if (tiles) {
-        load(0);
-        store(0, 0);
-        there = there_next;
+    uint32_t there = ALL;
+    if (tiles > 0) {
+        load(0, stage);
+        store(0, 0, stage);
+        there = stage.there;
+        if (tiles > 1) load(1, stage);
     }
+    // Tile `tile` is in LDS, the next one in registers or on its way there.  Behind the first product, while the matrix units still work on it, that one is
+    // stored and the one behind it sets out: in front, its eight loads held back the product's LDS reads; at the end, the stores were waited for.
     for (int tile = 0; tile < tiles; ++tile) {
         const int buf = tile & 1, kv = tile * KT;
         __syncthreads();
-        if (tile + 1 < tiles) load(tile + 1);
-        if (kv <= lim_last) {
-            f32x16 s[KB];
+        const bool live = kv <= lim_last;
+        f32x16 s[KB];
+        if (live) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) s[kb] = (f32x16)0.f;
 #pragma unroll
             for (int st = 0; st < DS; ++st)
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) s[kb] = mfma32(*(const x8 *)(ks[buf] + (32 * kb + (lane & 31)) * KLD + 16 * st + 8 * h), qf[st], s[kb]);
-            const bool masked = kv + KT - 1 > lim_first || (PAGED && (there & ((1u << (KT / 16)) - 1)) != (1u << (KT / 16)) - 1);
+                for (int kb = 0; kb < KB; ++kb) s[kb] = mfma32(*(const x8 *)(ks[buf] + (32 * (kb0 + kb) + (lane & 31)) * KLD + 16 * st + 8 * h), qf[st], s[kb]);
+        }
+        const uint32_t there_next = stage.there;
+        if (tile + 1 < tiles) store(buf ^ 1, tile + 1, stage);
+        if (tile + 2 < tiles) load(tile + 2, stage);
+        if (live) {
+            const bool masked = kv + KT - 1 > lim_first || (PAGED && there != ALL);
             auto seen = [&](int kb, int r) {              // register r of block kb: key 32 kb + 8 (r / 4) + 4 h + r % 4
-                return kv + 32 * kb + 8 * (r >> 2) + 4 * h + (r & 3) <= lim && (!PAGED || (there >> (2 * kb + (r >> 3)) & 1));
+                return kv + 32 * (kb0 + kb) + 8 * (r >> 2) + 4 * h + (r & 3) <= lim && (!PAGED || (there >> (2 * (kb0 + kb) + (r >> 3)) & 1));
             };
             if (masked)
 #pragma unroll
@@ -239,14 +284,33 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
 #pragma unroll
             for (int i = 0; i < 2 * KB; ++i)
 #pragma unroll
-                for (int d = 0; d < DB; ++d) o[d] = mfma32(read_vt<T, VLD>(vs[buf], 16 * i, 32 * d, lane), p[i >> 1][i & 1], o[d]);
+                for (int d = 0; d < DB; ++d) o[d] = mfma32(read_vt<T, VLD>(vs[buf], 32 * kb0 + 16 * i, 32 * d, lane), p[i >> 1][i & 1], o[d]);
         }
-        if (tile + 1 < tiles) {
-            store(buf ^ 1, tile + 1);
-            there = there_next;
-        }
+        there = there_next;
     }
-    const float l = sum_halves((ls[0] + ls[1]) + (ls[2] + ls[3]));
+    float l = (ls[0] + ls[1]) + (ls[2] + ls[3]);
+    if constexpr (KS == 2) {             // the two waves' parts of 32 rows: the second leaves its own in LDS
+        static_assert(sizeof(ks) >= RW * 64 * (16 * DB + 2) * 4, "the parts fit where K was");
+        float *part = (float *)ks + wave % RW * 64 * (16 * DB + 2) + lane;
+        __syncthreads();
+        if (kb0) {
+#pragma unroll
+            for (int d = 0; d < DB; ++d)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) part[(16 * d + r) * 64] = o[d][r];
+            part[16 * DB * 64] = m, part[(16 * DB + 1) * 64] = l;
+        }
+        __syncthreads();
+        if (kb0) return;
+        const float m2 = part[16 * DB * 64], l2 = part[(16 * DB + 1) * 64], M = fmaxf(m, m2);
+        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M), f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - M);
+        l = l * f + l2 * f2;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[d][r] = o[d][r] * f + part[(16 * d + r) * 64] * f2;
+    }
+    l = sum_halves(l);
     if (!valid) return;
     const float inv = l == 0 ? 0.f : 1 / l;
     if (tiles && odd)
@@ -278,23 +342,35 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
         }
 }
 
-template <typename T, bool PAGED>
-static hipError_t prompt_launch(const AttnArgs &a, hipStream_t st) {
-    const int n_head_kv = a.n_head / a.group;
-    const int64_t blocks = ((int64_t)a.n_q * a.group / PR_ROWS + a.n_seq) * n_head_kv;   // every sequence may end inside a block
+// Two waves for 32 rows where there are few workgroups: a tile then takes a wave 1.3 us instead of 1.6, and there are twice as many.  512 rows behind
+// 1536, 32 heads of 128 in f16 (128 blocks): 51 -> 42 us; 1000 rows, 32/8 heads in bf16 (256): 30 -> 27; but 2048, 32/32 (544): 60 -> 64 and 4096,
+// 32/8 (1032): 170 -> 202: each wave's share of a tile's loads and waits is as large as before.
+constexpr int FEW_BLOCKS = 512;
+
+template <typename T, bool PAGED, int KS>
+static hipError_t prompt_launch(const AttnArgs &a, int64_t blocks, hipStream_t st) {
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
     const dim3 g((unsigned)blocks);
-    if (a.head_dim <= 32) attn_prompt_k<T, 32, PAGED><<<g, 256, 0, st>>>(a);
-    else if (a.head_dim <= 64) attn_prompt_k<T, 64, PAGED><<<g, 256, 0, st>>>(a);
-    else attn_prompt_k<T, 128, PAGED><<<g, 256, 0, st>>>(a);
+    if (a.head_dim <= 32) attn_prompt_k<T, 32, PAGED, KS><<<g, 256, 0, st>>>(a);
+    else if (a.head_dim <= 64) attn_prompt_k<T, 64, PAGED, KS><<<g, 256, 0, st>>>(a);
+    else attn_prompt_k<T, 128, PAGED, KS><<<g, 256, 0, st>>>(a);
     return hipGetLastError();
+}
+
+template <typename T, bool PAGED>
+static hipError_t prompt_rows(const AttnArgs &a, hipStream_t st) {
+    const int64_t rows = (int64_t)a.n_q * a.group, n_head_kv = a.n_head / a.group;
+    const int64_t blocks = (rows / 128 + a.n_seq) * n_head_kv;         // every sequence may end inside a block
+    if constexpr (sizeof(T) == 2)
+        if (blocks < FEW_BLOCKS) return prompt_launch<T, PAGED, 2>(a, (rows / 64 + a.n_seq) * n_head_kv, st);
+    return prompt_launch<T, PAGED, 1>(a, blocks, st);
 }
 
 hipError_t attn_prompt(const AttnArgs &a, int type, bool paged, hipStream_t st) {
     switch (type) {
-        case FL_TYPE_F32: return paged ? prompt_launch<float, true>(a, st) : prompt_launch<float, false>(a, st);
-        case FL_TYPE_F16: return paged ? prompt_launch<h16, true>(a, st) : prompt_launch<h16, false>(a, st);
-        default: return paged ? prompt_launch<b16, true>(a, st) : prompt_launch<b16, false>(a, st);
+        case FL_TYPE_F32: return paged ? prompt_rows<float, true>(a, st) : prompt_rows<float, false>(a, st);
+        case FL_TYPE_F16: return paged ? prompt_rows<h16, true>(a, st) : prompt_rows<h16, false>(a, st);
+        default: return paged ? prompt_rows<b16, true>(a, st) : prompt_rows<b16, false>(a, st);
     }
 }
 

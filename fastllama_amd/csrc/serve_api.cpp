@@ -95,6 +95,7 @@ static int fill(AttnArgs &a, const char *fn, int type, int head_dim, int n_head,
     if (n_head < 1 || n_head > 65535 || n_head % n_head_kv) return set_error(FL_EINVAL, "%s: %d query heads over %d key heads", fn, n_head, n_head_kv);
     if (!(scale > 0) || !std::isfinite(scale)) return set_error(FL_EINVAL, "%s: scale %g is not a positive number", fn, (double)scale);
     if (n_seq < 0) return set_error(FL_EINVAL, "%s: %d sequences", fn, n_seq);
+    if ((int64_t)n_q * n_head > INT32_MAX) return set_error(FL_EINVAL, "%s: %d rows of %d heads: more than 2^31", fn, n_q, n_head);
     FL_TRY(check_heads(fn, "q", q, type, n_q));
     FL_TRY(check_out(fn, "out", out, type, n_q, n_head));
     a.q = q->data_dev, a.q_ld = q->token_stride, a.q_hs = q->head_stride;
@@ -122,7 +123,7 @@ int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scal
 
 size_t fl_attn_pages_workspace(const fl_kv_pages *c, int n_head, int n_table, int n_seq) {
     if (!c || c->n_head_kv < 1 || n_head < 1 || n_table < 1 || n_seq < 1 || c->page_size < 1) return 0;
-    return attn_decode_workspace(n_seq, n_head, c->n_head_kv, c->head_dim, (int64_t)n_table * c->page_size);
+    return attn_decode_workspace(c->type, n_seq, n_head, c->n_head_kv, c->head_dim, (int64_t)n_table * c->page_size);
 }
 
 int fl_attn_pages(const fl_kv_pages *c, int n_head, float scale, const fl_heads *q, int n_q, const int32_t *cu_q_dev, const int32_t *kv_len_dev,

@@ -193,41 +193,51 @@ _TYPES = {torch.float32: hip.F32, torch.float16: hip.F16, torch.bfloat16: hip.BF
 
 
 def _type(t: torch.Tensor, what: str) -> int:
-    if not (t.dtype in _TYPES):
+    n = _TYPES.get(t.dtype)
+    if n is None:
         raise _Error(f"{what}: {t.dtype} is not float32, float16 or bfloat16")
-    return _TYPES[t.dtype]
+    return n
 
 
-def _here(t: torch.Tensor, device: int, what: str) -> None:
-    """The kernels run on the current device's current stream."""
-    if not (isinstance(t, torch.Tensor) and t.is_cuda):
-        raise _Error(f"{what}: expected a device tensor: fastllama_amd has no CPU path")
-    if not (t.get_device() == device):
-        raise _Error(f"{what} is on {t.device}, the current device is cuda:{device}")
+def _elsewhere(t, device: int, what: str) -> Exception:
+    """The kernels run on the current device's current stream: why a tensor that is not there is refused."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        return _Error(f"{what}: expected a device tensor: fastllama_amd has no CPU path")
+    return _Error(f"{what} is on {t.device}, the current device is cuda:{device}")
 
 
 def _heads(t: torch.Tensor, device: int, what: str) -> hip.Heads:
     """[rows, heads, head_dim] of any strides, the last axis dense"""
-    _here(t, device, what)
-    if not (t.dim() == 3 and (t.stride(2) == 1 or t.shape[2] == 1)):
-        raise _Error(f"{what}: want [rows, heads, head_dim] with a dense last axis, got {tuple(t.shape)} strides {t.stride()}")
-    n, h, _ = t.shape
-    return hip.Heads(t.data_ptr(), t.stride(0) if n > 1 else 0, t.stride(1) if h > 1 else 0)
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        raise _elsewhere(t, device, what)
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 3 or (stride[2] != 1 and shape[2] != 1):
+        raise _Error(f"{what}: want [rows, heads, head_dim] with a dense last axis, got {tuple(shape)} strides {stride}")
+    return hip.Heads(t.data_ptr(), stride[0] if shape[0] > 1 else 0, stride[1] if shape[1] > 1 else 0)
 
 
-def _index(t: torch.Tensor, device: int, what: str, n: int) -> int:
-    _here(t, device, what)
-    if not (t.dtype == torch.int32 and t.dim() == 1 and t.shape[0] == n and (n < 2 or t.stride(0) == 1)):
-        raise _Error(f"{what}: want {n} dense int32, got {tuple(t.shape)} {t.dtype}")
+def _row(t: torch.Tensor, device: int, what: str, n: int, dtype: torch.dtype = torch.int32) -> int:
+    """The address of n dense values."""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        raise _elsewhere(t, device, what)
+    shape = t.shape
+    if t.dtype != dtype or len(shape) != 1 or shape[0] != n or (n > 1 and t.stride(0) != 1):
+        raise _Error(f"{what}: want {n} dense {dtype}, got {tuple(shape)} {t.dtype}")
     return t.data_ptr()
 
 
-def _table(t: torch.Tensor, device: int) -> tuple[int, int]:
-    """(address, row stride) of [sequences, pages]"""
-    _here(t, device, "table")
-    if not (t.dtype == torch.int32 and t.dim() == 2 and (t.shape[1] < 2 or t.stride(1) == 1)):
-        raise _Error(f"table: want int32 [sequences, pages] with a dense last axis, got {tuple(t.shape)} {t.dtype}")
-    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else t.shape[1]
+def _table(t: torch.Tensor, device: int) -> tuple[int, int, int, int]:
+    """(address, row stride, sequences, pages) of [sequences, pages]"""
+    if not isinstance(t, torch.Tensor) or t.get_device() != device:
+        raise _elsewhere(t, device, "table")
+    shape, stride = t.shape, t.stride()
+    if t.dtype != torch.int32 or len(shape) != 2 or (shape[1] > 1 and stride[1] != 1):
+        raise _Error(f"table: want int32 [sequences, pages] with a dense last axis, got {tuple(shape)} {t.dtype}")
+    return t.data_ptr(), stride[0] if shape[0] > 1 else shape[1], shape[0], shape[1]
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 class KVPages:
@@ -256,7 +266,7 @@ class KVPages:
         return cls(torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
 
     def check(self, device: int) -> None:
-        if not (self.device == device):
+        if self.device != device:
             raise _Error(f"the cache is on cuda:{self.device}, the current device is cuda:{device}")
 
 
@@ -265,20 +275,20 @@ def kv_append(pages: KVPages, k: torch.Tensor, v: torch.Tensor, table: torch.Ten
     sequences: rows cu[b]..cu[b+1]-1, or one row for each sequence where cu is None.  No two rows of a call may go to one slot."""
     device, d = torch.cuda.current_device(), pages.desc
     pages.check(device)
-    if not (k.shape == v.shape and k.dtype == v.dtype and k.dim() == 3 and k.shape[1] == d.n_head_kv and k.shape[2] == d.head_dim):
-        raise _Error(f"k, v: want [rows, {d.n_head_kv}, {d.head_dim}] alike, got {tuple(k.shape)} and {tuple(v.shape)}")
-    kh, vh, (tab, ld) = _heads(k, device, "k"), _heads(v, device, "v"), _table(table, device)
-    n = table.shape[0]
-    if not (cu is not None or n == k.shape[0]):
-        raise _Error(f"{k.shape[0]} rows for {n} sequences and no row starts")
-    check(hip.load().fl_kv_append(pages.ref, _type(k, "k"), C.byref(kh), C.byref(vh), k.shape[0], None if cu is None else _index(cu, device, "cu", n + 1),
-                                  _index(n_past, device, "n_past", n), tab, ld, table.shape[1], n, _stream()), "fl_kv_append")
+    kh, vh, (tab, ld, n, width) = _heads(k, device, "k"), _heads(v, device, "v"), _table(table, device)
+    shape = k.shape
+    if shape != v.shape or k.dtype != v.dtype or shape[1] != d.n_head_kv or shape[2] != d.head_dim:
+        raise _Error(f"k, v: want [rows, {d.n_head_kv}, {d.head_dim}] alike, got {tuple(shape)} and {tuple(v.shape)}")
+    if cu is None and n != shape[0]:
+        raise _Error(f"{shape[0]} rows for {n} sequences and no row starts")
+    check(hip.load().fl_kv_append(pages.ref, _type(k, "k"), kh, vh, shape[0], None if cu is None else _row(cu, device, "cu", n + 1),
+                                  _row(n_past, device, "n_past", n), tab, ld, width, n, _raw_stream(device)), "fl_kv_append")
 
 
 def _out(q: torch.Tensor, out: torch.Tensor | None) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if not (out.shape == q.shape and out.dtype == q.dtype):
+    if out.shape != q.shape or out.dtype != q.dtype:
         raise _Error(f"out: want {tuple(q.shape)} {q.dtype}, got {tuple(out.shape)} {out.dtype}")
     return out
 
@@ -290,18 +300,17 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
     one less; one that sees none becomes 0.  Rows outside every sequence are not written.  scale: 1 / sqrt(head_dim) unless given."""
     device = torch.cuda.current_device()
     qh, kh, vh = _heads(q, device, "q"), _heads(k, device, "k"), _heads(v, device, "v")
-    if not (k.shape == v.shape and k.shape[2] == q.shape[2] and q.dtype == k.dtype == v.dtype):
-        raise _Error(f"q, k, v: {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit together")
-    _here(cu_q, device, "cu_q")
+    qs, ks = q.shape, k.shape
+    if ks != v.shape or ks[2] != qs[2] or not q.dtype == k.dtype == v.dtype:
+        raise _Error(f"q, k, v: {tuple(qs)} {q.dtype}, {tuple(ks)} {k.dtype}, {tuple(v.shape)} {v.dtype} do not fit together")
     n = cu_q.numel() - 1
-    if not (n >= 0 and (cu_kv is not None or q.shape[0] == k.shape[0])):
+    if n < 0 or (cu_kv is None and qs[0] != ks[0]):
         raise _Error("cu_q is empty, or other numbers of rows and keys and no cu_kv")
-    cu = _index(cu_q, device, "cu_q", n + 1)
+    cu = _row(cu_q, device, "cu_q", n + 1)
     out = _out(q, out)
-    oh = _heads(out, device, "out")
-    check(hip.load().fl_attn_prompt(_type(q, "q"), q.shape[2], q.shape[1], k.shape[1], q.shape[2] ** -0.5 if scale is None else scale, C.byref(qh), q.shape[0],
-                                    C.byref(kh), C.byref(vh), k.shape[0], cu, cu if cu_kv is None else _index(cu_kv, device, "cu_kv", n + 1), n, C.byref(oh),
-                                    _stream()), "fl_attn_prompt")
+    check(hip.load().fl_attn_prompt(_type(q, "q"), qs[2], qs[1], ks[1], qs[2] ** -0.5 if scale is None else scale, qh, qs[0], kh, vh, ks[0], cu,
+                                    cu if cu_kv is None else _row(cu_kv, device, "cu_kv", n + 1), n, _heads(out, device, "out"), _raw_stream(device)),
+          "fl_attn_prompt")
     return out
 
 
@@ -311,19 +320,19 @@ def attn_pages(q: torch.Tensor, pages: KVPages, table: torch.Tensor, kv_len: tor
     sequence (its newest token), or with ``cu_q`` the rows cu_q[b]..cu_q[b+1]-1 of each (its newest tokens, already in the cache)."""
     device, d = torch.cuda.current_device(), pages.desc
     pages.check(device)
-    qh, (tab, ld) = _heads(q, device, "q"), _table(table, device)
-    n = table.shape[0]
-    if not (q.dtype == pages.k.dtype and q.shape[2] == d.head_dim):
+    qh, (tab, ld, n, width) = _heads(q, device, "q"), _table(table, device)
+    rows, heads, dim = q.shape
+    if q.dtype != pages.k.dtype or dim != d.head_dim:
         raise _Error(f"q: {tuple(q.shape)} {q.dtype} does not fit a cache of head_dim {d.head_dim}, {pages.k.dtype}")
-    if not (cu_q is not None or n == q.shape[0]):
-        raise _Error(f"{q.shape[0]} rows for {n} sequences and no row starts")
-    lens, cu = _index(kv_len, device, "kv_len", n), None if cu_q is None else _index(cu_q, device, "cu_q", n + 1)
+    if cu_q is None and n != rows:
+        raise _Error(f"{rows} rows for {n} sequences and no row starts")
+    lens, cu = _row(kv_len, device, "kv_len", n), None if cu_q is None else _row(cu_q, device, "cu_q", n + 1)
     out = _out(q, out)
-    oh, lib = _heads(out, device, "out"), hip.load()
-    size = 0 if cu_q is not None else lib.fl_attn_pages_workspace(pages.ref, q.shape[1], table.shape[1], n)
+    lib = hip.load()
+    size = 0 if cu_q is not None else lib.fl_attn_pages_workspace(pages.ref, heads, width, n)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
-    check(lib.fl_attn_pages(pages.ref, q.shape[1], d.head_dim ** -0.5 if scale is None else scale, C.byref(qh), q.shape[0], cu, lens, tab, ld, table.shape[1], n,
-                            C.byref(oh), ws.data_ptr() if size else None, size, _stream()), "fl_attn_pages")
+    check(lib.fl_attn_pages(pages.ref, heads, dim ** -0.5 if scale is None else scale, qh, rows, cu, lens, tab, ld, width, n, _heads(out, device, "out"),
+                            ws.data_ptr() if size else None, size, _raw_stream(device)), "fl_attn_pages")
     return out
 
 
@@ -331,25 +340,20 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     """A token (int32 [rows]) for each row of ``logits`` [rows, n_vocab] from the uniform numbers ``u`` [rows] in [0, 1).  Each setting is a number
     for all rows or a device tensor of one for each (float32; top_k int32).  Off: top_k <= 0, top_p >= 1, min_p <= 0; temperature <= 0 is greedy."""
     device = torch.cuda.current_device()
-    _here(logits, device, "logits")
-    if not (logits.dim() == 2 and (logits.stride(1) == 1 or logits.shape[1] == 1)):
-        raise _Error(f"logits: want [rows, n_vocab] with a dense last axis, got {tuple(logits.shape)}")
-    rows, vocab = logits.shape
+    if not isinstance(logits, torch.Tensor) or logits.get_device() != device:
+        raise _elsewhere(logits, device, "logits")
+    shape, stride = logits.shape, logits.stride()
+    if len(shape) != 2 or (stride[1] != 1 and shape[1] != 1):
+        raise _Error(f"logits: want [rows, n_vocab] with a dense last axis, got {tuple(shape)} strides {stride}")
+    rows, vocab = shape
     p = hip.SampleParams()
-
-    def per_row(t, what, dtype):
-        _here(t, device, what)
-        if not (t.dtype == dtype and t.dim() == 1 and t.shape[0] == rows and (rows < 2 or t.stride(0) == 1)):
-            raise _Error(f"{what}: want {rows} dense {dtype}, got {tuple(t.shape)} {t.dtype}")
-        return t.data_ptr()
-
     for what, x in (("temperature", temperature), ("top_p", top_p), ("min_p", min_p)):
         if isinstance(x, torch.Tensor):
-            setattr(p, what + "_dev", per_row(x, what, torch.float32))
+            setattr(p, what + "_dev", _row(x, device, what, rows, torch.float32))
         else:
             setattr(p, what, x)
     if isinstance(top_k, torch.Tensor):
-        p.top_k_dev = per_row(top_k, "top_k", torch.int32)
+        p.top_k_dev = _row(top_k, device, "top_k", rows)
     else:
         p.top_k = max(0, min(int(top_k), vocab))
     if out is None:
@@ -357,6 +361,6 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature=1.0, top_k=0, top_
     lib = hip.load()
     size = lib.fl_sample_workspace(rows, vocab)
     ws = torch.empty(size, dtype=torch.uint8, device=logits.device)
-    check(lib.fl_sample(_type(logits, "logits"), logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, rows, vocab, per_row(u, "u", torch.float32),
-                               C.byref(p), per_row(out, "out", torch.int32), ws.data_ptr(), size, _stream()), "fl_sample")
+    check(lib.fl_sample(_type(logits, "logits"), logits.data_ptr(), stride[0] if rows > 1 else vocab, rows, vocab, _row(u, device, "u", rows, torch.float32), p,
+                        _row(out, device, "out", rows), ws.data_ptr(), size, _raw_stream(device)), "fl_sample")
     return out
