@@ -3,7 +3,7 @@
 //   out[i][h] = sum_j exp(s_ij - max) v_j / sum_j exp(s_ij - max),  s_ij = scale q_i . k_j,  keys j <= lk - lq + i of i's own sequence
 //
 // The query heads that share a key head are rows of one problem: row r of (sequence, key head) is token r / group, head r % group, so a
-// workgroup's 128 rows read each key and value once for the whole group, and few tokens still fill a tile.  A wave has 32 rows; K and V pass
+// workgroup's rows read each key and value once for the whole group, and few tokens still fill a tile.  A wave has 32 rows; K and V pass
 // through LDS in tiles of KT keys, the next tile's loads in flight (registers) while this one is computed, two LDS tiles in turn: one barrier a tile.
 //
 // Both products are taken transposed: S^T = K Q^T leaves each lane a column, one query row with half of the tile's keys (lane and lane + 32
@@ -46,13 +46,13 @@ __device__ inline typename Vec<T>::x8 read_vt(const T *v, int row, int d0, int l
     return r;
 }
 
-// KS: waves that share 32 rows, each with its part of every tile's keys; they join at the end.
-template <typename T, int DP, bool PAGED, int KS>
-__global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
+// W waves; KS of them share 32 rows, each with its part of every tile's keys, and join at the end.
+template <typename T, int DP, bool PAGED, int KS, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
     typedef typename Vec<T>::x8 x8;
     constexpr int KT = Tile<T>::KT, KLD = DP + Tile<T>::KPAD, VLD = DP + Tile<T>::VPAD;
-    constexpr int UNIT = 16 / sizeof(T), CPR = DP / UNIT, RPP = 256 / CPR, PASSES = KT / RPP;   // 16-byte chunks of a row, rows of a pass over the tile
-    constexpr int KB = KT / 32 / KS, DB = DP / 32, DS = DP / 16, RW = 4 / KS, PR_ROWS = 32 * RW;   // KB blocks of 32 keys a wave, RW waves of rows
+    constexpr int UNIT = 16 / sizeof(T), CPR = DP / UNIT, RPP = 64 * W / CPR, PASSES = KT / RPP;   // 16-byte chunks of a row, rows of a pass over the tile
+    constexpr int KB = KT / 32 / KS, DB = DP / 32, DS = DP / 16, RW = W / KS, PR_ROWS = 32 * RW;   // KB blocks of 32 keys a wave, RW waves of rows
     static_assert(KT % RPP == 0 && PASSES >= 1, "a tile is whole passes of the workgroup");
     __shared__ __attribute__((aligned(16))) T ks[2][KT * KLD], vs[2][KT * VLD];
 
@@ -342,36 +342,39 @@ __global__ __launch_bounds__(256, 2) void attn_prompt_k(AttnArgs a) {
         }
 }
 
-// Two waves for 32 rows where there are few workgroups: a tile then takes a wave 1.3 us instead of 1.6, and there are twice as many.  512 rows behind
-// 1536, 32 heads of 128 in f16 (128 blocks): 51 -> 42 us; 1000 rows, 32/8 heads in bf16 (256): 30 -> 27; but 2048, 32/32 (544): 60 -> 64 and 4096,
-// 32/8 (1032): 170 -> 202: each wave's share of a tile's loads and waits is as large as before.
-constexpr int FEW_BLOCKS = 512;
-
-template <typename T, bool PAGED, int KS>
-static hipError_t prompt_launch(const AttnArgs &a, int64_t blocks, hipStream_t st) {
+template <typename T, int DP, bool PAGED, int KS, int W>
+static hipError_t prompt_launch(const AttnArgs &a, hipStream_t st) {
+    const int64_t rows = (int64_t)a.n_q * a.group, blocks = (rows / (32 * W / KS) + a.n_seq) * (a.n_head / a.group);   // every sequence may end inside a block
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    const dim3 g((unsigned)blocks);
-    if (a.head_dim <= 32) attn_prompt_k<T, 32, PAGED, KS><<<g, 256, 0, st>>>(a);
-    else if (a.head_dim <= 64) attn_prompt_k<T, 64, PAGED, KS><<<g, 256, 0, st>>>(a);
-    else attn_prompt_k<T, 128, PAGED, KS><<<g, 256, 0, st>>>(a);
+    attn_prompt_k<T, DP, PAGED, KS, W><<<dim3((unsigned)blocks), 64 * W, 0, st>>>(a);
     return hipGetLastError();
 }
 
-template <typename T, bool PAGED>
+// Few workgroups (16-bit types): two waves for 32 rows.  A tile then takes a wave 1.3 us instead of 1.6, and there are twice as many workgroups: 512
+// rows behind 1536, 32 heads of 128 in f16 (128 blocks of 128 rows) 51 -> 42 us; 1000 rows, 32/8 heads in bf16 (256) 30 -> 27; but 2048, 32/32 (544)
+// 60 -> 64 and 4096, 32/8 (1032) 170 -> 202: each wave's share of a tile's loads and waits is as large as before.
+// Many: eight waves, which load a tile once for 256 rows: 8192 rows, 32/8 heads (1024 blocks of 256) 577 -> 542 us, 4096 (512) 174 -> 160; but 2048, 32/32
+// (256, one for each CU) 61 -> 68.
+template <typename T, int DP, bool PAGED>
 static hipError_t prompt_rows(const AttnArgs &a, hipStream_t st) {
     const int64_t rows = (int64_t)a.n_q * a.group, n_head_kv = a.n_head / a.group;
-    const int64_t blocks = (rows / 128 + a.n_seq) * n_head_kv;         // every sequence may end inside a block
-    if constexpr (sizeof(T) == 2)
-        if (blocks < FEW_BLOCKS) return prompt_launch<T, PAGED, 2>(a, (rows / 64 + a.n_seq) * n_head_kv, st);
-    return prompt_launch<T, PAGED, 1>(a, blocks, st);
+    if constexpr (sizeof(T) == 2) {
+        if ((rows / 128 + a.n_seq) * n_head_kv < 512) return prompt_launch<T, DP, PAGED, 2, 4>(a, st);
+        if constexpr (DP == 128 && !PAGED)
+            if (rows / 256 * n_head_kv >= 512) return prompt_launch<T, DP, PAGED, 1, 8>(a, st);
+    }
+    return prompt_launch<T, DP, PAGED, 1, 4>(a, st);
+}
+
+template <typename T>
+static hipError_t prompt_dim(const AttnArgs &a, bool paged, hipStream_t st) {
+    if (a.head_dim <= 32) return paged ? prompt_rows<T, 32, true>(a, st) : prompt_rows<T, 32, false>(a, st);
+    if (a.head_dim <= 64) return paged ? prompt_rows<T, 64, true>(a, st) : prompt_rows<T, 64, false>(a, st);
+    return paged ? prompt_rows<T, 128, true>(a, st) : prompt_rows<T, 128, false>(a, st);
 }
 
 hipError_t attn_prompt(const AttnArgs &a, int type, bool paged, hipStream_t st) {
-    switch (type) {
-        case FL_TYPE_F32: return paged ? prompt_rows<float, true>(a, st) : prompt_rows<float, false>(a, st);
-        case FL_TYPE_F16: return paged ? prompt_rows<h16, true>(a, st) : prompt_rows<h16, false>(a, st);
-        default: return paged ? prompt_rows<b16, true>(a, st) : prompt_rows<b16, false>(a, st);
-    }
+    return type == FL_TYPE_F32 ? prompt_dim<float>(a, paged, st) : type == FL_TYPE_F16 ? prompt_dim<h16>(a, paged, st) : prompt_dim<b16>(a, paged, st);
 }
 
 }  // namespace fl
