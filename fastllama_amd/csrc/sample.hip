@@ -93,6 +93,7 @@ __device__ inline u64 target_of(float u, u64 total) {
 constexpr int BINS = 2048, SHORT = 256, WAVES = S_THREADS / 64, CAP = 8192;
 constexpr int ROUND = 4096, P_CAP = 512;     // logits that a part's workgroup has in registers at a time; candidates of a part
 constexpr int FEW = 128;                     // "small" top_k: half of a part's threads
+constexpr int COARSE = P_THREADS;            // bins, one a thread, for a part's own cut
 
 struct Part {
     uint32_t kmax, first, held, pad;         // the largest key, its first index, candidates (may be more than P_CAP)
@@ -256,7 +257,7 @@ __device__ inline uint32_t row_max(const Work &w, int parts) {
 
 template <typename T>
 __global__ __launch_bounds__(P_THREADS) void sample_scan_k(SampleArgs a, int part_len, int parts) {
-    __shared__ uint32_t hist[BINS];
+    __shared__ uint32_t hist[COARSE];
     __shared__ u64 sums[P_THREADS / 64], found[2];
     __shared__ int counts[P_THREADS / 64];
     __shared__ u64 best[P_THREADS / 64];
@@ -267,7 +268,7 @@ __global__ __launch_bounds__(P_THREADS) void sample_scan_k(SampleArgs a, int par
     const int p0 = p * part_len, p1 = min(p0 + part_len, r.n);
     const bool few = set.few && !set.greedy;
     if (few)
-        for (int i = t; i < BINS; i += P_THREADS) hist[i] = 0;
+        hist[t] = 0;
     else
         for (int i = p * P_THREADS + t; i < BINS; i += parts * P_THREADS) w.hist[i] = 0;
     float mine = -INFINITY;                  // this thread's largest, and where it stands first
@@ -291,15 +292,14 @@ __global__ __launch_bounds__(P_THREADS) void sample_scan_k(SampleArgs a, int par
     if (few && kmax) {
         const Bins bins(value_of(kmax), set.temp);
         const uint32_t own = bins(mine);
-        if (own < BINS) atomicAdd(&hist[own], 1u);
+        if (own < BINS) atomicAdd(&hist[own / (BINS / COARSE)], 1u);
         __syncthreads();
-        constexpr int PER = BINS / P_THREADS;
-        u64 v[PER], before;
+        u64 before;
         uint32_t bin;
-        for (int i = 0; i < PER; ++i) v[i] = hist[t * PER + i];
+        const u64 v[1] = {hist[t]};
         // where fewer threads than top_k are in range, the last bin: all that can have a weight
-        scan_bins<PER, P_THREADS>(v, sums, found, [&](u64) { return (u64)set.top_k; }, &bin, &before);
-        held = compact(r, p0, p1, bins, 0, bin, w.list + (size_t)p * P_CAP, counts, [](float) {});
+        scan_bins<1, P_THREADS>(v, sums, found, [&](u64) { return (u64)set.top_k; }, &bin, &before);
+        held = compact(r, p0, p1, bins, 0, min(bin * (BINS / COARSE) + BINS / COARSE - 1, (uint32_t)BINS - 1), w.list + (size_t)p * P_CAP, counts, [](float) {});
     }
     if (t == 0) w.part[p].kmax = kmax, w.part[p].first = ~(uint32_t)b, w.part[p].held = held;
 }
@@ -750,6 +750,8 @@ __global__ __launch_bounds__(S_THREADS) void sample_draw_k(SampleArgs a, PowerTa
     else rest(Whole<T>(r, weigh, 0, r.n));
 }
 
+constexpr int MAX_ROWS = 2048;               // of a launch
+
 // Parts of one round while that makes at most 2048 workgroups, of up to four rounds beyond: fewer of them join their bins.
 static int part_rounds(int rows, int n_vocab) {
     const int64_t blocks = (int64_t)rows * ((n_vocab + ROUND - 1) / ROUND);
@@ -760,7 +762,7 @@ static int part_count(int rows, int n_vocab) {
     return (n_vocab + len - 1) / len;
 }
 
-size_t sample_workspace(int rows, int n_vocab) { return rows * Work::row_bytes(part_count(rows, n_vocab)); }
+size_t sample_workspace(int rows, int n_vocab) { return min(rows, MAX_ROWS) * Work::row_bytes(part_count(rows, n_vocab)); }
 
 template <typename T>
 static hipError_t sample_launch(const SampleArgs &a, hipStream_t st) {
@@ -773,10 +775,10 @@ static hipError_t sample_launch(const SampleArgs &a, hipStream_t st) {
     // what the host knows of all rows
     const bool greedy = !a.temperature_p && !(a.temperature > 0), few = !a.top_k_p && a.top_k > 0 && a.top_k < a.n_vocab && a.top_k <= FEW;
     const bool cuts = a.top_k_p || a.top_p_p || (a.top_k > 0 && a.top_k < a.n_vocab) || a.top_p < 1;
-    for (int row = 0; row < a.rows; row += 65535) {                    // (the grid's second axis)
+    for (int row = 0; row < a.rows; row += MAX_ROWS) {                 // (one after the other on the stream, in the same workspace)
         SampleArgs b = a;
-        const int rows = b.rows = min(a.rows - row, 65535);
-        b.logits = (const T *)a.logits + row * a.ld, b.u += row, b.tokens += row, b.ws = (char *)a.ws + row * Work::row_bytes(parts);
+        const int rows = b.rows = min(a.rows - row, MAX_ROWS);
+        b.logits = (const T *)a.logits + row * a.ld, b.u += row, b.tokens += row;
         if (b.temperature_p) b.temperature_p += row;
         if (b.top_k_p) b.top_k_p += row;
         if (b.top_p_p) b.top_p_p += row;

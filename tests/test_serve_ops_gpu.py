@@ -430,6 +430,16 @@ def test_sample_strided_rows_and_unaligned(ops):
     assert torch.equal(ops.sample(wide[:, 5:1008], u, 0.8, 40, 0.95), want)
 
 
+def test_sample_more_rows_than_one_launch_takes(ops):
+    l = logits_like(9, 4500, 300, F32)
+    u, t = torch.rand(4500, device="cuda"), torch.rand(4500, device="cuda") + 0.2
+    k, p = torch.randint(0, 300, (4500,), device="cuda").int(), torch.rand(4500, device="cuda") + 0.3
+    got = ops.sample(l, u, t, k, p, 0.01)
+    for a in range(0, 4500, 900):
+        b = slice(a, a + 900)
+        assert torch.equal(got[b], ops.sample(l[b], u[b], t[b], k[b], p[b], 0.01))
+
+
 def test_sample_follows_the_distribution(ops):
     """65536 evenly spaced u: each token comes up in its share of them, within the two ends of its stretch."""
     V, n = 50, 1 << 16
