@@ -19,7 +19,6 @@
 
 namespace fl {
 
-
 template <typename T>
 struct Tile {                            // LDS tiles of a type
     static constexpr int KT = sizeof(T) == 2 ? 64 : 32, KPAD = 16 / sizeof(T), VPAD = sizeof(T) == 2 ? 32 : 4;
@@ -46,28 +45,19 @@ __device__ inline typename Vec<T>::x8 read_vt(const T *v, int row, int d0, int l
     return r;
 }
 
-// W waves; KS of them share 32 rows, each with its part of every tile's keys, and join at the end.
-template <typename T, int DP, bool PAGED, int KS, int W>
-__global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
-    typedef typename Vec<T>::x8 x8;
-    constexpr int KT = Tile<T>::KT, KLD = DP + Tile<T>::KPAD, VLD = DP + Tile<T>::VPAD;
-    constexpr int UNIT = 16 / sizeof(T), CPR = DP / UNIT, RPP = 64 * W / CPR, PASSES = KT / RPP;   // 16-byte chunks of a row, rows of a pass over the tile
-    constexpr int KB = KT / 32 / KS, DB = DP / 32, DS = DP / 16, RW = W / KS, PR_ROWS = 32 * RW;   // KB blocks of 32 keys a wave, RW waves of rows
-    static_assert(KT % RPP == 0 && PASSES >= 1, "a tile is whole passes of the workgroup");
-    __shared__ __attribute__((aligned(16))) T ks[2][KT * KLD], vs[2][KT * VLD];
-
-    __shared__ int odd;
-    if (threadIdx.x == 0) odd = 0;
-    __syncthreads();
-
-    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, kb0 = wave / RW * KB, n_head_kv = a.n_head / a.group;
-    // Workgroups go round the 8 XCDs by their number: with 8 key heads (or a multiple) all that read a head's keys share an L2.
-    const int hk = blockIdx.x % n_head_kv;
-    int blk = blockIdx.x / n_head_kv, b = -1, q0 = 0, lq = 0;
+// A workgroup's block of rows: sequence b has rows q0 .. q0 + lq - 1 and lk keys (packed ones from k0 on); the block is its number blk.  All values are
+// the same in all threads.  b = -1: there is none.
+struct Block {
+    int b, q0, lq, k0, lk, blk;
+};
+template <bool PAGED, int ROWS>
+__device__ Block find_block(const AttnArgs &a, int blk, int blocks) {
+    const int lane = threadIdx.x & 63;
+    int b = -1, q0 = 0, lq = 0;
     auto blocks_of = [&](int s, int *f, int *e) {                      // sequence s's first row and end; returns its blocks
         *f = *e = 0;
         if (s < a.n_seq) seq_rows(a.cu_q, s, a.n_q, f, e);
-        return (int)(((int64_t)(*e - *f) * a.group + PR_ROWS - 1) / PR_ROWS);
+        return (int)(((int64_t)(*e - *f) * a.group + ROWS - 1) / ROWS);
     };
     if (a.n_seq <= 64) {
         // The longest ways first, or the last to start ends long behind the others: a block's number in its sequence is (but for keys of the past) its
@@ -89,12 +79,12 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
                 blk -= c;
             }
         }
-        if (level < 0) return;
+        if (level < 0) return Block{-1, 0, 0, 0, 0, 0};
         const unsigned long long has = __ballot(n > level);
         const int w = __builtin_ctzll(__ballot(n > level && __popcll(has & ((1ull << lane) - 1)) == blk));
         b = w, q0 = __builtin_amdgcn_readlane(f, w), lq = __builtin_amdgcn_readlane(e, w) - q0, blk = level;
     } else {
-        blk = gridDim.x / n_head_kv - 1 - blk;
+        blk = blocks - 1 - blk;
         for (int s0 = 0; s0 < a.n_seq; s0 += 64) {                     // 64 sequences at a time
             int f, e;
             const int n = blocks_of(s0 + lane, &f, &e);
@@ -112,7 +102,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
             blk -= total;
         }
     }
-    if (b < 0) return;
+    if (b < 0) return Block{-1, 0, 0, 0, 0, 0};
     int k0 = 0, lk;
     if (PAGED) lk = (int)min(max(a.kv_len[b], 0), a.n_table << a.page_shift);
     else {
@@ -120,12 +110,47 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
         seq_rows(a.cu_kv, b, a.n_kv, &k0, &k1);
         lk = k1 - k0;
     }
+    return Block{b, q0, lq, k0, lk, blk};
+}
+
+// The tiles of a block of rows whose last row sees `end` keys, cut into parts of at least four: part `part` has tiles *t0 .. *t1 - 1.  Returns the number
+// of parts that have any (0 keys: 1).
+template <int KT>
+__device__ inline int cut_tiles(int end, int parts, int part, int *t0, int *t1) {
+    const int tiles = end > 0 ? (end + KT - 1) / KT : 0, n = max(1, min(parts, tiles / 4)), per = (tiles + n - 1) / n;
+    *t0 = min(part * per, tiles), *t1 = min(*t0 + per, tiles);
+    return tiles ? (tiles + per - 1) / per : 1;
+}
+
+// W waves; KS of them share 32 rows, each with its part of every tile's keys, and join at the end.
+template <typename T, int DP, bool PAGED, int KS, int W>
+__global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a, int parts) {
+    typedef typename Vec<T>::x8 x8;
+    constexpr int KT = Tile<T>::KT, KLD = DP + Tile<T>::KPAD, VLD = DP + Tile<T>::VPAD;
+    constexpr int UNIT = 16 / sizeof(T), CPR = DP / UNIT, RPP = 64 * W / CPR, PASSES = KT / RPP;   // 16-byte chunks of a row, rows of a pass over the tile
+    constexpr int KB = KT / 32 / KS, DB = DP / 32, DS = DP / 16, RW = W / KS, PR_ROWS = 32 * RW;   // KB blocks of 32 keys a wave, RW waves of rows
+    static_assert(KT % RPP == 0 && PASSES >= 1, "a tile is whole passes of the workgroup");
+    __shared__ __attribute__((aligned(16))) T ks[2][KT * KLD], vs[2][KT * VLD];
+
+    __shared__ int odd;
+    if (threadIdx.x == 0) odd = 0;
+    __syncthreads();
+
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6), h = lane >> 5, kb0 = wave / RW * KB, n_head_kv = a.n_head / a.group;
+    // Workgroups go round the 8 XCDs by their number: with 8 key heads (or a multiple) all that read a head's keys share an L2.
+    const int hk = blockIdx.x % n_head_kv;
+    const Block at = find_block<PAGED, PR_ROWS>(a, blockIdx.x / n_head_kv, gridDim.x / n_head_kv);
+    if (at.b < 0) return;
+    const int b = at.b, q0 = at.q0, lq = at.lq, k0 = at.k0, lk = at.lk, blk = at.blk;
     const int D = a.head_dim, rows = lq * a.group, r0 = blk * PR_ROWS, rw = r0 + wave % RW * 32, row = rw + (lane & 31);
     const bool valid = row < rows;
     const int tok = (valid ? row : rows - 1) / a.group, head = hk * a.group + (valid ? row : rows - 1) % a.group;
     const int past = lk - lq, lim = past + tok;                    // the last key that this lane's row sees
     const int lim_first = past + min(rw, rows - 1) / a.group, lim_last = past + min(rw + 31, rows - 1) / a.group;   // of the wave's rows
-    const int end = min(past + min(r0 + PR_ROWS - 1, rows - 1) / a.group + 1, lk), tiles = end > 0 ? (end + KT - 1) / KT : 0;
+    const int end = min(past + min(r0 + PR_ROWS - 1, rows - 1) / a.group + 1, lk);
+    int t0, tiles;                                                     // of this part; `tiles` ends it
+    const int used = cut_tiles<KT>(end, parts, blockIdx.y, &t0, &tiles);
+    if ((int)blockIdx.y >= used) return;
 
     x8 qf[DS];
     {
@@ -156,8 +181,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
     auto load = [&](int tile, Stage &to) {
         to.there = ALL;
         if constexpr (PAGED) {
-            if (tile % BATCH == 0) {
-                const int j = (tile * BLOCKS + lane) * 16, p = j < end ? table[j >> a.page_shift] : -1;
+            if (tile == t0 || tile % BATCH == 0) {
+                const int j = (tile / BATCH * 64 + lane) * 16, p = j < end ? table[j >> a.page_shift] : -1;
                 pages = p >= 0 && p < a.n_pages ? p : -1;
             }
             to.there = (uint32_t)(__ballot(pages >= 0) >> (tile % BATCH * BLOCKS)) & ALL;
@@ -223,15 +248,15 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
     for (int d = 0; d < DB; ++d) o[d] = (f32x16)0.f;
     float m = -INFINITY, ls[4] = {0, 0, 0, 0};                        // the sum in four chains
     uint32_t there = ALL;
-    if (tiles > 0) {
-        load(0, stage);
-        store(0, 0, stage);
+    if (tiles > t0) {
+        load(t0, stage);
+        store(t0 & 1, t0, stage);
         there = stage.there;
-        if (tiles > 1) load(1, stage);
+        if (tiles > t0 + 1) load(t0 + 1, stage);
     }
     // Tile `tile` is in LDS, the next one in registers or on its way there.  Behind the first product, while the matrix units still work on it, that one is
     // stored and the one behind it sets out: in front, its eight loads held back the product's LDS reads; at the end, the stores were waited for.
-    for (int tile = 0; tile < tiles; ++tile) {
+    for (int tile = t0; tile < tiles; ++tile) {
         const int buf = tile & 1, kv = tile * KT;
         __syncthreads();
         const bool live = kv <= lim_last;
@@ -304,7 +329,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
         if (kb0) return;
         const float m2 = part[16 * DB * 64], l2 = part[(16 * DB + 1) * 64], M = fmaxf(m, m2);
         const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M), f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - M);
-        l = l * f + l2 * f2;
+        l = l * f + l2 * f2, m = M;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
 #pragma unroll
@@ -312,9 +337,8 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
     }
     l = sum_halves(l);
     if (!valid) return;
-    const float inv = l == 0 ? 0.f : 1 / l;
-    if (tiles && odd)
-        for (int j = max(whole, 0) / KT * KT; j <= min(lim, end - 1); ++j) {
+    if (tiles > t0 && odd)
+        for (int j = max(max(whole, 0) / KT, t0) * KT; j <= min(lim, min(end, tiles * KT) - 1); ++j) {
             int64_t vo = (int64_t)(k0 + j) * a.v_ld;
             if (PAGED) {
                 const int p = table[j >> a.page_shift];
@@ -330,6 +354,16 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
                     if (at < D && !finite(v[at])) o[d][r] += (float)v[at];
                 }
         }
+    if (used > 1) {                      // this part's sums of the row, for attn_prompt_join_k
+        float *to = (float *)a.ws + (((int64_t)(q0 + tok) * a.n_head + head) * parts + blockIdx.y) * (DP + 4);
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) *(f32x4 *)(to + 32 * d + 2 * r + 4 * h) = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+        if (h == 0) to[DP] = m, to[DP + 1] = l;
+        return;
+    }
+    const float inv = l == 0 ? 0.f : 1 / l;
     T *out = (T *)a.out + (int64_t)(q0 + tok) * a.o_ld + head * a.o_hs;
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -342,11 +376,43 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a) {
         }
 }
 
+// The rows whose keys were cut into parts: the same blocks, four rows at a time, 64 threads for a row.
+template <typename T, int DP, bool PAGED, int ROWS>
+__global__ __launch_bounds__(256) void attn_prompt_join_k(AttnArgs a, int parts) {
+    const int n_head_kv = a.n_head / a.group, hk = blockIdx.x % n_head_kv, lane = threadIdx.x & 63, D = a.head_dim;
+    const Block at = find_block<PAGED, ROWS>(a, blockIdx.x / n_head_kv, gridDim.x / n_head_kv);
+    if (at.b < 0) return;
+    const int rows = at.lq * a.group, r0 = at.blk * ROWS, past = at.lk - at.lq;
+    const int end = min(past + min(r0 + ROWS - 1, rows - 1) / a.group + 1, at.lk);
+    int t0, t1;
+    const int used = cut_tiles<Tile<T>::KT>(end, parts, 0, &t0, &t1);
+    if (used == 1) return;
+    for (int row = r0 + blockIdx.y * 4 + (threadIdx.x >> 6); row < min(r0 + ROWS, rows); row += 4 * gridDim.y) {
+        const int tok = row / a.group, head = hk * a.group + row % a.group;
+        const float *part = (const float *)a.ws + ((int64_t)(at.q0 + tok) * a.n_head + head) * parts * (DP + 4);
+        float M = -INFINITY, l = 0, sum[2] = {0, 0};
+        for (int s = 0; s < used; ++s) M = fmaxf(M, part[s * (DP + 4) + DP]);
+#pragma unroll 4
+        for (int s = 0; s < used; ++s) {
+            const float *p = part + s * (DP + 4);
+            const float m = p[DP], ls = p[DP + 1], x = p[min(lane, DP - 1)], y = p[min(lane + 64, DP - 1)];
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+            l += f == 0 ? 0.f : ls * f, sum[0] += f == 0 ? 0.f : x * f, sum[1] += f == 0 ? 0.f : y * f;
+        }
+        T *out = (T *)a.out + (int64_t)(at.q0 + tok) * a.o_ld + head * a.o_hs;
+        const float inv = l == 0 ? 0.f : 1 / l;
+        if (lane < D) out[lane] = (T)(sum[0] * inv);
+        if (lane + 64 < D) out[lane + 64] = (T)(sum[1] * inv);
+    }
+}
+
 template <typename T, int DP, bool PAGED, int KS, int W>
-static hipError_t prompt_launch(const AttnArgs &a, hipStream_t st) {
-    const int64_t rows = (int64_t)a.n_q * a.group, blocks = (rows / (32 * W / KS) + a.n_seq) * (a.n_head / a.group);   // every sequence may end inside a block
+static hipError_t prompt_launch(const AttnArgs &a, int parts, hipStream_t st) {
+    constexpr int ROWS = 32 * W / KS;
+    const int64_t rows = (int64_t)a.n_q * a.group, blocks = (rows / ROWS + a.n_seq) * (a.n_head / a.group);   // every sequence may end inside a block
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
-    attn_prompt_k<T, DP, PAGED, KS, W><<<dim3((unsigned)blocks), 64 * W, 0, st>>>(a);
+    attn_prompt_k<T, DP, PAGED, KS, W><<<dim3((unsigned)blocks, parts), 64 * W, 0, st>>>(a, parts);
+    if (parts > 1) attn_prompt_join_k<T, DP, PAGED, ROWS><<<dim3((unsigned)blocks, 8), 256, 0, st>>>(a, parts);
     return hipGetLastError();
 }
 
@@ -355,15 +421,30 @@ static hipError_t prompt_launch(const AttnArgs &a, hipStream_t st) {
 // 60 -> 64 and 4096, 32/8 (1032) 170 -> 202: each wave's share of a tile's loads and waits is as large as before.
 // Many: eight waves, which load a tile once for 256 rows: 8192 rows, 32/8 heads (1024 blocks of 256) 577 -> 542 us, 4096 (512) 174 -> 160; but 2048, 32/32
 // (256, one for each CU) 61 -> 68.
+// Very few, behind many keys: the keys too are cut into parts of four tiles or more, until each CU has two workgroups, and joined by a second launch.  64
+// rows behind 30000, 32/8 heads of 128 in bf16: 575 -> 79 us (105 at one workgroup a CU); 16 behind 2000 in f16: 47 -> 20 (25 with parts of eight
+// tiles); 200 behind 1600, 8 heads in f32: 249 -> 44; 512 behind 1536, 32/32 in f16 (two parts): 51 -> 51.
+static bool few_blocks(int type, int64_t rows, int64_t n_head_kv, int n_seq) { return type != FL_TYPE_F32 && (rows / 128 + n_seq) * n_head_kv < 512; }
+static int prompt_parts(int type, int64_t rows, int64_t n_head_kv, int n_seq, int64_t max_keys) {
+    const int tile = type == FL_TYPE_F32 ? 32 : 64, block = few_blocks(type, rows, n_head_kv, n_seq) ? 64 : 128;
+    const int64_t blocks = (rows + block - 1) / block * n_head_kv;
+    return (int)max((int64_t)1, min(min((int64_t)16, 512 / max(blocks, (int64_t)1)), max_keys / (4 * tile)));
+}
+size_t attn_prompt_workspace(int type, int n_q, int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_keys) {
+    const int parts = prompt_parts(type, (int64_t)n_q * (n_head / n_head_kv), n_head_kv, n_seq, max_keys);
+    return parts > 1 ? (size_t)n_q * n_head * parts * ((head_dim <= 32 ? 32 : head_dim <= 64 ? 64 : 128) + 4) * 4 : 0;
+}
+
 template <typename T, int DP, bool PAGED>
 static hipError_t prompt_rows(const AttnArgs &a, hipStream_t st) {
     const int64_t rows = (int64_t)a.n_q * a.group, n_head_kv = a.n_head / a.group;
+    const int type = sizeof(T) == 4 ? FL_TYPE_F32 : FL_TYPE_F16, parts = prompt_parts(type, rows, n_head_kv, a.n_seq, PAGED ? (int64_t)a.n_table << a.page_shift : a.n_kv);
     if constexpr (sizeof(T) == 2) {
-        if ((rows / 128 + a.n_seq) * n_head_kv < 512) return prompt_launch<T, DP, PAGED, 2, 4>(a, st);
+        if (few_blocks(type, rows, n_head_kv, a.n_seq)) return prompt_launch<T, DP, PAGED, 2, 4>(a, parts, st);
         if constexpr (DP == 128 && !PAGED)
-            if (rows / 256 * n_head_kv >= 512) return prompt_launch<T, DP, PAGED, 1, 8>(a, st);
+            if (rows / 256 * n_head_kv >= 512) return prompt_launch<T, DP, PAGED, 1, 8>(a, 1, st);
     }
-    return prompt_launch<T, DP, PAGED, 1, 4>(a, st);
+    return prompt_launch<T, DP, PAGED, 1, 4>(a, parts, st);
 }
 
 template <typename T>

@@ -105,8 +105,19 @@ static int fill(AttnArgs &a, const char *fn, int type, int head_dim, int n_head,
     return FL_OK;
 }
 
+static int check_workspace(const char *fn, const char *query, size_t need, const void *ws, size_t bytes) {
+    if (need && (!ws || bytes < need || !aligned(ws, 16)))
+        return set_error(FL_EINVAL, "%s: a workspace of %zu bytes, aligned to 16 (want %zu: %s)", fn, ws ? bytes : 0, need, query);
+    return FL_OK;
+}
+
+size_t fl_attn_prompt_workspace(int type, int head_dim, int n_head, int n_head_kv, int n_q, int n_kv, int n_seq) {
+    if (!size_of(type) || head_dim < 1 || n_head_kv < 1 || n_head < n_head_kv || n_q < 1 || n_kv < 1 || n_seq < 1) return 0;
+    return attn_prompt_workspace(type, n_q, n_seq, n_head, n_head_kv, head_dim, n_kv);
+}
+
 int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scale, const fl_heads *q, int n_q, const fl_heads *k, const fl_heads *v, int n_kv,
-                   const int32_t *cu_q_dev, const int32_t *cu_kv_dev, int n_seq, const fl_heads *out, void *stream) {
+                   const int32_t *cu_q_dev, const int32_t *cu_kv_dev, int n_seq, const fl_heads *out, void *workspace_dev, size_t workspace_bytes, void *stream) {
     const char *fn = "fl_attn_prompt";
     AttnArgs a{};
     FL_TRY(fill(a, fn, type, head_dim, n_head, n_head_kv, scale, q, out, n_q, n_seq));
@@ -114,6 +125,8 @@ int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scal
     FL_TRY(check_heads(fn, "v", v, type, n_kv));
     if (n_q == 0 || n_seq == 0) return FL_OK;
     if (!cu_q_dev || !cu_kv_dev) return set_error(FL_EINVAL, "%s: null row starts", fn);
+    FL_TRY(check_workspace(fn, "fl_attn_prompt_workspace", fl_attn_prompt_workspace(type, head_dim, n_head, n_head_kv, n_q, n_kv, n_seq), workspace_dev, workspace_bytes));
+    a.ws = workspace_dev;
     FL_TRY(ensure_device());
     a.k = k->data_dev, a.v = v->data_dev, a.k_ld = k->token_stride, a.k_hs = k->head_stride, a.v_ld = v->token_stride, a.v_hs = v->head_stride;
     a.cu_q = cu_q_dev, a.cu_kv = cu_kv_dev, a.n_kv = n_kv;
@@ -121,8 +134,9 @@ int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scal
     return e == hipSuccess ? FL_OK : hip_fail(e, fn);
 }
 
-size_t fl_attn_pages_workspace(const fl_kv_pages *c, int n_head, int n_table, int n_seq) {
-    if (!c || c->n_head_kv < 1 || n_head < 1 || n_table < 1 || n_seq < 1 || c->page_size < 1) return 0;
+size_t fl_attn_pages_workspace(const fl_kv_pages *c, int n_head, int n_q, int n_table, int n_seq, int one_row) {
+    if (!c || !size_of(c->type) || c->head_dim < 1 || c->n_head_kv < 1 || n_head < c->n_head_kv || n_q < 1 || n_table < 1 || n_seq < 1 || c->page_size < 1) return 0;
+    if (!one_row) return attn_prompt_workspace(c->type, n_q, n_seq, n_head, c->n_head_kv, c->head_dim, (int64_t)n_table * c->page_size);
     return attn_decode_workspace(c->type, n_seq, n_head, c->n_head_kv, c->head_dim, (int64_t)n_table * c->page_size);
 }
 
@@ -137,12 +151,8 @@ int fl_attn_pages(const fl_kv_pages *c, int n_head, float scale, const fl_heads 
     if (!kv_len_dev || (!cu_q_dev && n_seq != n_q)) return set_error(FL_EINVAL, "%s: no lengths, or no row starts for %d rows of %d sequences", fn, n_q, n_seq);
     a.k = c->k_dev, a.v = c->v_dev, a.k_ld = a.v_ld = c->slot_stride, a.k_hs = a.v_hs = c->head_stride, a.page_stride = c->page_stride;
     a.cu_q = cu_q_dev, a.kv_len = kv_len_dev, a.table = table_dev, a.table_ld = table_ld, a.n_table = n_table, a.page_shift = page_shift(c), a.n_pages = c->n_pages;
-    if (!cu_q_dev) {
-        const size_t need = fl_attn_pages_workspace(c, n_head, n_table, n_seq);
-        if (need && (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16)))
-            return set_error(FL_EINVAL, "%s: a workspace of %zu bytes, aligned to 16 (want %zu: fl_attn_pages_workspace)", fn, workspace_dev ? workspace_bytes : 0, need);
-        a.ws = workspace_dev;
-    }
+    FL_TRY(check_workspace(fn, "fl_attn_pages_workspace", fl_attn_pages_workspace(c, n_head, n_q, n_table, n_seq, !cu_q_dev), workspace_dev, workspace_bytes));
+    a.ws = workspace_dev;
     FL_TRY(ensure_device());
     const hipError_t e = cu_q_dev ? attn_prompt(a, c->type, true, S(stream)) : attn_decode(a, c->type, S(stream));
     return e == hipSuccess ? FL_OK : hip_fail(e, fn);
@@ -159,9 +169,7 @@ int fl_sample(int type, const void *logits_dev, int64_t ld, int rows, int n_voca
     if (rows == 0) return FL_OK;
     if (!logits_dev || !u_dev || !p || !tokens_dev) return set_error(FL_EINVAL, "%s: null argument", fn);
     if (!aligned(logits_dev, (size_t)size_of(type))) return set_error(FL_EINVAL, "%s: logits not aligned to their type", fn);
-    const size_t need = sample_workspace(rows, n_vocab);
-    if (!workspace_dev || workspace_bytes < need || !aligned(workspace_dev, 16))
-        return set_error(FL_EINVAL, "%s: a workspace of %zu bytes, aligned to 16 (want %zu: fl_sample_workspace)", fn, workspace_dev ? workspace_bytes : 0, need);
+    FL_TRY(check_workspace(fn, "fl_sample_workspace", sample_workspace(rows, n_vocab), workspace_dev, workspace_bytes));
     FL_TRY(ensure_device());
     SampleArgs a{};
     a.logits = logits_dev, a.ld = ld, a.rows = rows, a.n_vocab = n_vocab, a.u = u_dev, a.tokens = tokens_dev, a.ws = workspace_dev;

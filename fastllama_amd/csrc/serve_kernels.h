@@ -46,6 +46,7 @@ struct SampleArgs {
 };
 
 hipError_t attn_prompt(const AttnArgs &a, int type, bool paged, hipStream_t st);
+size_t attn_prompt_workspace(int type, int n_q, int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_keys);
 hipError_t attn_decode(const AttnArgs &a, int type, hipStream_t st);
 size_t attn_decode_workspace(int type, int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_len);
 hipError_t kv_append(const AppendArgs &a, int src_type, int type, hipStream_t st);

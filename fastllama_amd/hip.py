@@ -108,8 +108,9 @@ _PROTOS = {
     "fl_kv_append": (C.c_int, [C.POINTER(KVPagesDesc), C.c_int, C.POINTER(Heads), C.POINTER(Heads), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p,
                                C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "fl_attn_prompt": (C.c_int, [C.c_int, C.c_int, C.c_int, C.c_int, C.c_float, C.POINTER(Heads), C.c_int, C.POINTER(Heads), C.POINTER(Heads),
-                                 C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(Heads), C.c_void_p]),
-    "fl_attn_pages_workspace": (C.c_size_t, [C.POINTER(KVPagesDesc), C.c_int, C.c_int, C.c_int]),
+                                 C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.POINTER(Heads), C.c_void_p, C.c_size_t, C.c_void_p]),
+    "fl_attn_prompt_workspace": (C.c_size_t, [C.c_int] * 7),
+    "fl_attn_pages_workspace": (C.c_size_t, [C.POINTER(KVPagesDesc)] + [C.c_int] * 5),
     "fl_attn_pages": (C.c_int, [C.POINTER(KVPagesDesc), C.c_int, C.c_float, C.POINTER(Heads), C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int,
                                 C.c_int, C.c_int, C.POINTER(Heads), C.c_void_p, C.c_size_t, C.c_void_p]),
     "fl_sample": (C.c_int, [C.c_int, C.c_void_p, C.c_int64, C.c_int, C.c_int, C.c_void_p, C.POINTER(SampleParams), C.c_void_p,

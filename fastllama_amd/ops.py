@@ -308,9 +308,12 @@ def attn_prompt(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.T
         raise _Error("cu_q is empty, or other numbers of rows and keys and no cu_kv")
     cu = _row(cu_q, device, "cu_q", n + 1)
     out = _out(q, out)
-    check(hip.load().fl_attn_prompt(_type(q, "q"), qs[2], qs[1], ks[1], qs[2] ** -0.5 if scale is None else scale, qh, qs[0], kh, vh, ks[0], cu,
-                                    cu if cu_kv is None else _row(cu_kv, device, "cu_kv", n + 1), n, _heads(out, device, "out"), _raw_stream(device)),
-          "fl_attn_prompt")
+    lib, kind = hip.load(), _type(q, "q")
+    size = lib.fl_attn_prompt_workspace(kind, qs[2], qs[1], ks[1], qs[0], ks[0], n)
+    ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
+    check(lib.fl_attn_prompt(kind, qs[2], qs[1], ks[1], qs[2] ** -0.5 if scale is None else scale, qh, qs[0], kh, vh, ks[0], cu,
+                             cu if cu_kv is None else _row(cu_kv, device, "cu_kv", n + 1), n, _heads(out, device, "out"), ws.data_ptr() if size else None, size,
+                             _raw_stream(device)), "fl_attn_prompt")
     return out
 
 
@@ -329,7 +332,7 @@ def attn_pages(q: torch.Tensor, pages: KVPages, table: torch.Tensor, kv_len: tor
     lens, cu = _row(kv_len, device, "kv_len", n), None if cu_q is None else _row(cu_q, device, "cu_q", n + 1)
     out = _out(q, out)
     lib = hip.load()
-    size = 0 if cu_q is not None else lib.fl_attn_pages_workspace(pages.ref, heads, width, n)
+    size = lib.fl_attn_pages_workspace(pages.ref, heads, rows, width, n, cu_q is None)
     ws = torch.empty(size, dtype=torch.uint8, device=q.device) if size else None
     check(lib.fl_attn_pages(pages.ref, heads, dim ** -0.5 if scale is None else scale, qh, rows, cu, lens, tab, ld, width, n, _heads(out, device, "out"),
                             ws.data_ptr() if size else None, size, _raw_stream(device)), "fl_attn_pages")

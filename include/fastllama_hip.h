@@ -182,14 +182,15 @@ typedef struct {
 int fl_kv_append(const fl_kv_pages *c, int src_type, const fl_heads *k, const fl_heads *v, int n_tokens, const int32_t *cu_dev,
                  const int32_t *n_past_dev, const int32_t *table_dev, int table_ld, int n_table, int n_seq, void *stream);
 /* Causal attention over packed prompts: rows cu_q[b].. of q see the keys cu_kv[b].. of their own sequence; the last row sees all of them and each row
- * before it one less (more keys than rows: positions that were there before).  A row that sees no key becomes 0. */
+ * before it one less (more keys than rows: positions that were there before).  A row that sees no key becomes 0.  Few rows behind many keys are split over
+ * the keys and joined, for which the caller keeps a workspace of fl_attn_prompt_workspace() bytes (0: none) that no other call uses at the same time. */
+size_t fl_attn_prompt_workspace(int type, int head_dim, int n_head, int n_head_kv, int n_q, int n_kv, int n_seq);
 int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scale, const fl_heads *q, int n_q, const fl_heads *k, const fl_heads *v, int n_kv,
-                   const int32_t *cu_q_dev, const int32_t *cu_kv_dev, int n_seq, const fl_heads *out, void *stream);
+                   const int32_t *cu_q_dev, const int32_t *cu_kv_dev, int n_seq, const fl_heads *out, void *workspace_dev, size_t workspace_bytes, void *stream);
 /* The same over a cache: sequence b has positions 0..kv_len[b]-1 in the pages table[b][...] (row stride table_ld, n_table pages each).  cu_q_dev
- * NULL: one row for each sequence, the newest token; the work is split over long caches and joined, for which the caller keeps a workspace of
- * fl_attn_pages_workspace() bytes (0: none) that no other call uses at the same time.  Otherwise cu_q gives the rows of each sequence, the
- * newest kv_len[b] positions' last, and no workspace is used. */
-size_t fl_attn_pages_workspace(const fl_kv_pages *c, int n_head, int n_table, int n_seq);
+ * NULL: one row for each sequence, the newest token (one_row != 0 in the query); otherwise cu_q gives the rows of each sequence, the newest of its
+ * kv_len[b] positions.  A workspace as above. */
+size_t fl_attn_pages_workspace(const fl_kv_pages *c, int n_head, int n_q, int n_table, int n_seq, int one_row);
 int fl_attn_pages(const fl_kv_pages *c, int n_head, float scale, const fl_heads *q, int n_q, const int32_t *cu_q_dev, const int32_t *kv_len_dev,
                   const int32_t *table_dev, int table_ld, int n_table, int n_seq, const fl_heads *out, void *workspace_dev, size_t workspace_bytes,
                   void *stream);

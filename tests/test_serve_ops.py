@@ -50,8 +50,8 @@ def test_append_refuses(L):
     assert append(L, n=0, k=heads(None), v=heads(None)) == hip.FL_OK            # nothing to do
 
 
-def prompt(L, type=hip.F16, D=64, H=4, Hkv=2, scale=0.1, q=None, nq=9, k=None, v=None, nk=9, cq=P, ck=P, ns=2, out=None):
-    return L.fl_attn_prompt(type, D, H, Hkv, scale, q or heads(ts=256), nq, k or heads(), v or heads(), nk, cq, ck, ns, out or heads(ts=256), None)
+def prompt(L, type=hip.F16, D=64, H=4, Hkv=2, scale=0.1, q=None, nq=9, k=None, v=None, nk=9, cq=P, ck=P, ns=2, out=None, ws=P, size=1 << 40):
+    return L.fl_attn_prompt(type, D, H, Hkv, scale, q or heads(ts=256), nq, k or heads(), v or heads(), nk, cq, ck, ns, out or heads(ts=256), ws, size, None)
 
 
 def test_prompt_refuses(L):
@@ -69,7 +69,7 @@ def pages(L, c=None, H=4, scale=0.1, q=None, nq=2, cu=None, lens=P, table=P, ld=
 
 
 def test_pages_refuses(L):
-    assert pages(L) == GOOD and pages(L, nq=9, cu=P, ws=None, size=0) == GOOD
+    assert pages(L) == GOOD and pages(L, nq=9, cu=P) == GOOD
     for kw in BAD_CACHES:
         assert pages(L, cache(**kw)) == hip.FL_EINVAL, kw
     for kw in (dict(H=3), dict(H=0), dict(scale=0.0), dict(q=heads(None)), dict(nq=3), dict(nq=-1), dict(lens=None), dict(table=None), dict(nt=0), dict(ld=4),
@@ -82,12 +82,26 @@ def test_pages_refuses(L):
 def test_pages_workspace(L):
     """What the query names is enough, anything less is refused, also where it is not aligned."""
     for H, nt, ns in ((4, 5, 2), (4, 4096, 1), (64, 256, 64), (2, 100000, 3)):
-        size = L.fl_attn_pages_workspace(cache(), H, nt, ns)
+        size = L.fl_attn_pages_workspace(cache(), H, ns, nt, ns, 1)
         assert pages(L, H=H, nq=ns, ld=nt, nt=nt, ns=ns, size=size, ws=P if size else None) == GOOD
         if size:
             for kw in (dict(size=size - 1), dict(ws=None), dict(ws=P + 4)):
                 assert pages(L, **{**dict(H=H, nq=ns, ld=nt, nt=nt, ns=ns, size=size), **kw}) == hip.FL_EINVAL
-    assert L.fl_attn_pages_workspace(None, 4, 5, 2) == 0 and L.fl_attn_pages_workspace(cache(), 0, 5, 2) == 0
+    assert L.fl_attn_pages_workspace(None, 4, 2, 5, 2, 1) == 0 and L.fl_attn_pages_workspace(cache(), 0, 2, 5, 2, 1) == 0
+    seen = 0
+    for H, nq, n in ((4, 9, 40), (2, 16, 30000), (4, 100, 5000), (64, 5000, 5000)):     # several rows a sequence; prompts
+        size = L.fl_attn_pages_workspace(cache(), H, nq, n // 16, 3, 0)
+        kw = dict(H=H, nq=nq, cu=P, ld=n, nt=n // 16, ns=3)
+        assert pages(L, **kw, size=size, ws=P if size else None) == GOOD
+        also = L.fl_attn_prompt_workspace(hip.F16, 64, H, 2, nq, n, 3)
+        kp = dict(H=H, nq=nq, nk=n, ns=3)
+        assert prompt(L, **kp, size=also, ws=P if also else None) == GOOD
+        for f, need, k in ((pages, size, kw), (prompt, also, kp)):
+            if need:
+                seen += 1
+                for bad in (dict(size=need - 1), dict(ws=None), dict(ws=P + 4)):
+                    assert f(L, **{**k, "size": need, **bad}) == hip.FL_EINVAL
+    assert seen >= 2 and L.fl_attn_prompt_workspace(2, 64, 4, 2, 9, 9, 1) == 0
 
 
 def sample(L, type=hip.F32, l=P, ld=100, rows=2, V=100, u=P, p=C.byref(hip.SampleParams()), out=P, ws=P, size=1 << 40):

@@ -124,6 +124,24 @@ def test_prompt_long(ops, T, n):
 
 
 @pytest.mark.parametrize("T", TYPES)
+@pytest.mark.parametrize("H,Hkv,lq,lk", [(2, 1, [3], [5000]), (8, 2, [16, 1, 0, 70], [9000, 3000, 700, 70]), (5, 5, [1, 1], [4096, 513]), (1, 1, [129], [2600])])
+@pytest.mark.parametrize("pages", [0, 64])
+def test_prompt_few_rows_behind_many_keys(ops, T, H, Hkv, lq, lk, pages):
+    check_prompt(ops, T, H, Hkv, 64 if pages else 128, lq, lk, seed=H, pages=pages)
+
+
+@pytest.mark.parametrize("T", TYPES)
+def test_prompt_not_finite_behind_many_keys(ops, T):
+    """As above for keys cut into parts: the last row's last key holds a value that is not finite, the rows before it do not see it."""
+    q, k, v = randn(1, 4, 2, 64, dtype=T), randn(2, 4000, 1, 64, dtype=T), randn(3, 4000, 1, 64, dtype=T)
+    want, bound = attention64(q, k, v, 0.125)
+    v[-1] = float("nan")
+    got = ops.attn_prompt(q, k, v, i32([0, 4]), i32([0, 4000]))
+    near(got[:3], want[:3], bound[:3])
+    assert got[3].isnan().all()
+
+
+@pytest.mark.parametrize("T", TYPES)
 @pytest.mark.parametrize("scale", [0.01, 2.0])
 def test_prompt_flat_and_sharp_scores(ops, T, scale):
     check_prompt(ops, T, 2, 2, 128, [150, 70], [150, 200], seed=9, scale=scale)
