@@ -93,7 +93,7 @@ int fl_kv_append(const fl_kv_pages *c, int src_type, const fl_heads *k, const fl
 static int fill(AttnArgs &a, const char *fn, int type, int head_dim, int n_head, int n_head_kv, float scale, const fl_heads *q, const fl_heads *out, int n_q, int n_seq) {
     FL_TRY(check_dim(fn, type, head_dim, n_head_kv));
     if (n_head < 1 || n_head > 65535 || n_head % n_head_kv) return set_error(FL_EINVAL, "%s: %d query heads over %d key heads", fn, n_head, n_head_kv);
-    if (!(scale > 0) || !std::isfinite(scale)) return set_error(FL_EINVAL, "%s: scale %g is not a positive number", fn, (double)scale);
+    if (!(scale > 0) || !std::isfinite(scale * 1.44269504088896341f)) return set_error(FL_EINVAL, "%s: scale %g is not a positive number", fn, (double)scale);
     if (n_seq < 0) return set_error(FL_EINVAL, "%s: %d sequences", fn, n_seq);
     if ((int64_t)n_q * n_head > INT32_MAX) return set_error(FL_EINVAL, "%s: %d rows of %d heads: more than 2^31", fn, n_q, n_head);
     FL_TRY(check_heads(fn, "q", q, type, n_q));

@@ -1,5 +1,5 @@
 """GPU: the operators over several sequences (paged cache, attention over prompts and pages, sampling) against plain 64-bit computations of their
-formulas.  Tolerances are bounds of the arithmetic, see attention_bound()."""
+formulas.  Tolerances are bounds of the arithmetic: attention64()."""
 import math
 
 import numpy as np
@@ -495,6 +495,34 @@ def test_model_logits_sample(ops):
     hip.check(call(5, 3))
     assert np.array_equal(got[5:8], want[5:8]) and (got[8:] == -9).all()
     assert call(0, 1 << 20) == hip.FL_EINVAL and call(n - 1, (1 << 31) - 1) == hip.FL_EINVAL
+
+
+def test_python_entry_points_refuse(ops):
+    """What the wrappers see on device tensors: shapes, types, strides and places that do not fit."""
+    from fastllama_amd import hip
+    d, host = torch.zeros(2, 2, 8, device="cuda"), torch.zeros(2, 2, 8)
+    cu, table, lens = i32([0, 2]), i32([[0], [1]]), i32([3, 4])
+    c = ops.KVPages.empty(4, 16, 2, 8, F32)
+    l, u = torch.zeros(2, 50, device="cuda"), torch.zeros(2, device="cuda")
+    ops.attn_prompt(d, d, d, cu), ops.attn_pages(d, c, table, lens), ops.kv_append(c, d, d, table, lens), ops.sample(l, u)
+    for bad in (lambda: ops.attn_prompt(host, d, d, cu), lambda: ops.attn_prompt(d, d.half(), d.half(), cu), lambda: ops.attn_prompt(d[0], d, d, cu),
+                lambda: ops.attn_prompt(d, d, d, cu.long()), lambda: ops.attn_prompt(d.double(), d.double(), d.double(), cu), lambda: ops.attn_prompt(d, d, d, cu.cpu()),
+                lambda: ops.attn_prompt(d, d, d, cu, out=d.half()), lambda: ops.attn_prompt(d.transpose(1, 2), d, d, cu), lambda: ops.attn_prompt(d, d[:1], d[:1], cu),
+                lambda: ops.attn_prompt(d, d, d, cu, i32([0, 1, 2])), lambda: ops.attn_prompt(d, d, d, cu, scale=-1.0), lambda: ops.attn_prompt(d, d, d, cu, scale=3e38),
+                lambda: ops.attn_prompt(d[:, :, :4].contiguous(), d[:, :, :4].contiguous(), d[:, :, :4].contiguous(), cu),
+                lambda: ops.attn_prompt(torch.zeros(40, device="cuda")[1:33].view(2, 2, 8), d, d, cu),              # not at 16 bytes
+                lambda: ops.attn_prompt(torch.zeros(2, 3, 8, device="cuda"), d, d, cu),                               # 3 heads over 2
+                lambda: ops.attn_prompt(d, d, d, cu, out=torch.zeros(1, 2, 8, device="cuda").expand(2, 2, 8)),
+                lambda: ops.attn_pages(d.half(), c, table, lens), lambda: ops.attn_pages(d, c, table[:1], lens), lambda: ops.attn_pages(d, c, table, lens[:1]),
+                lambda: ops.attn_pages(d, c, table.long(), lens), lambda: ops.attn_pages(d, c, i32([[0, 1], [2, 3]]).t(), lens), lambda: ops.attn_pages(d, c, table, lens, cu),
+                lambda: ops.kv_append(c, d, d[:1], table, lens), lambda: ops.kv_append(c, d.half(), d.half(), table, lens), lambda: ops.kv_append(c, d, d, table[:1], lens),
+                lambda: ops.KVPages(c.k, c.v[:2]), lambda: ops.KVPages(c.k, c.v.half()), lambda: ops.KVPages(c.k.cpu(), c.v), lambda: ops.KVPages(c.k[0], c.v[0]),
+                lambda: ops.attn_pages(d, ops.KVPages(c.k[:, :, :12], c.v[:, :, :12]), table, lens),                  # pages of 12
+                lambda: ops.sample(l.cpu(), u), lambda: ops.sample(l, u[:1]), lambda: ops.sample(l, u.double()), lambda: ops.sample(l.t(), u), lambda: ops.sample(l[0], u),
+                lambda: ops.sample(l, u, top_k=u), lambda: ops.sample(l, u, temperature=lens), lambda: ops.sample(l.int(), u), lambda: ops.sample(l[:, :0], u),
+                lambda: ops.sample(l, u, out=u)):
+        with pytest.raises(hip.FastLlamaHipError):
+            bad()
 
 
 # ------------------------------------------------------------------------------------------------ streams, graphs, together
