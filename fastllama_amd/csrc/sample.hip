@@ -186,6 +186,7 @@ __device__ u64 scan_bins(const u64 v[PER], u64 *sums, u64 *found, Need need_of, 
     if (t == 0) found[0] = BINS - 1, found[1] = 0;
     __syncthreads();
     u64 base = 0, total = 0;
+#pragma unroll 4
     for (int w = 0; w < N / 64; ++w) {
         if (w < t >> 6) base += sums[w];
         total += sums[w];
@@ -397,46 +398,30 @@ struct Shared {
     double table[32];
 };
 
-// What the cuts of one row are made from: the candidates in LDS, or all of a row.  Wave w has the stretch [i0, i1), in turns of 64.
-struct List {
+// What the cuts of one row are made from: the candidates in LDS, or all of a row.  Wave w has the stretch [i0, i1), in turns of 64.  (One code for both,
+// and the kernel below has each step once, in a loop: a launch fetches its instructions anew.  Against a form that had all steps twice, of 71 KB against
+// 22, 128 rows of 128256 took 28 us in place of 31, the call 87 in place of 91; rows whose logits are nearly all alike, which go to all of a row, took
+// 730 us in place of 630.)
+template <typename T>
+struct Source {
     Shared &s;
+    const Row<T> &r;
+    const Weigher &weigh;
+    bool list;
     int i0, i1;
-    __device__ List(Shared &s, int n) : s(s) {
+    __device__ Source(Shared &s, const Row<T> &r, const Weigher &weigh, bool list, int n) : s(s), r(r), weigh(weigh), list(list) {
         const int seg = ((n + WAVES - 1) / WAVES + 63) & ~63, wave = threadIdx.x >> 6;
         i0 = min(wave * seg, n), i1 = min(i0 + seg, n);
     }
-    __device__ uint32_t key(int i) const { return s.key[i]; }
-    __device__ u64 weight(int i, uint32_t) const { return s.weight[i]; }
-    __device__ int index(int i) const { return (int)s.idx[i]; }
+    __device__ uint32_t key(int i) const { return list ? s.key[i] : key_of((float)r.x[i]); }
+    __device__ u64 weight(int i, uint32_t key) const { return list ? s.weight[i] : weigh.of_key(key); }
+    __device__ int index(int i) const { return list ? (int)s.idx[i] : i; }
     template <typename F>
-    __device__ void each(F f) const {        // f(key, index, weight())
-        for (int i = i0 + (threadIdx.x & 63); i < i1; i += 64) f(s.key[i], (int)s.idx[i], [&] { return s.weight[i]; });
-    }
-};
-template <typename T>
-struct Whole {
-    const Row<T> &r;
-    const Weigher &weigh;
-    int i0, i1;
-    __device__ Whole(const Row<T> &r, const Weigher &weigh, int a, int b) : r(r), weigh(weigh) {
-        const int seg = ((b - a + WAVES - 1) / WAVES + 63) & ~63, wave = threadIdx.x >> 6;
-        i0 = min(a + wave * seg, b), i1 = min(i0 + seg, b);
-    }
-    __device__ uint32_t key(int i) const { return key_of((float)r.x[i]); }
-    __device__ u64 weight(int, uint32_t key) const { return weigh.of_key(key); }
-    __device__ int index(int i) const { return i; }
-    template <typename F>
-    __device__ void each(F f) const {
+    __device__ void each(F f) const {        // f(key, index, weight()) of those that are not -infinity
 #pragma unroll 1
-        for (int i = i0 + (threadIdx.x & 63); i < i1; i += 256) {
-            uint32_t x[4];                   // (four loads in flight)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[e] = i + 64 * e < i1 ? key(i + 64 * e) : 0;
-#pragma unroll 1
-            for (int e = 0; e < 4; ++e) {
-                const uint32_t k = e == 0 ? x[0] : e == 1 ? x[1] : e == 2 ? x[2] : x[3];
-                if (k) f(k, i + 64 * e, [&] { return weigh.of_key(k); });
-            }
+        for (int i = i0 + (threadIdx.x & 63); i < i1; i += 64) {
+            const uint32_t k = key(i);
+            if (k) f(k, index(i), [&] { return weight(i, k); });
         }
     }
 };
@@ -444,15 +429,15 @@ struct Whole {
 // The key at which the sum over the keys with in(), in falling order (of 1 each, or of the weights), reaches `need`: *tkey, and in *ties how many
 // equal keys that takes.  0 < need <= the sum over all.  A short list is ranked by comparing all with all; a long one (many logits within T / 64 of each
 // other) goes by the key's four bytes from the top.
-template <bool WEIGHTS, typename Src, typename In>
-__device__ void cut(Shared &s, const Src &src, u64 need, In in, uint32_t *tkey, u64 *ties) {
+template <typename Src, typename In>
+__device__ void cut(Shared &s, const Src &src, bool weights, u64 need, In in, uint32_t *tkey, u64 *ties) {
     const int t = threadIdx.x;
     if (t == 0) s.n = 0;
     __syncthreads();
     src.each([&](uint32_t k, int i, auto weight) {
         if (in(k)) {
             const uint32_t at = atomicAdd(&s.n, 1u);
-            if (at < SHORT) s.lkey[at] = k, s.lidx[at] = i, s.lw[at] = WEIGHTS ? weight() : 1;
+            if (at < SHORT) s.lkey[at] = k, s.lidx[at] = i, s.lw[at] = weights ? weight() : 1;
         }
     });
     __syncthreads();
@@ -468,7 +453,7 @@ __device__ void cut(Shared &s, const Src &src, u64 need, In in, uint32_t *tkey, 
                 const uint32_t kj = s.lkey[j], ij = s.lidx[j];
                 const u64 wj = s.lw[j];
                 const bool tie = (kj == key) & (ij < idx);
-                sum += (kj > key) | tie ? wj : 0;
+                sum += ((kj > key) | tie) ? wj : 0;
                 same += tie;
             }
             if (sum < need && sum + own >= need) s.prefix = key, s.need = same;
@@ -480,21 +465,24 @@ __device__ void cut(Shared &s, const Src &src, u64 need, In in, uint32_t *tkey, 
     }
     uint32_t prefix = 0, mask = 0;
     u64 left = need, unit = 1;
+#pragma unroll 1                             // (seldom run: small code, here and below; a launch fetches its instructions anew)
     for (int shift = 24; shift >= 0; shift -= 8) {
         if (t < 256) s.whist[t] = 0;
         if (t == 0) s.before = 1;
         __syncthreads();
         src.each([&](uint32_t k, int, auto weight) {
             if (((k ^ prefix) & mask) == 0 && in(k)) {
-                const u64 w = WEIGHTS ? weight() : 1;
+                const u64 w = weights ? weight() : 1;
                 if (w) atomicAdd(&s.whist[k >> shift & 255], w);
             }
         });
         __syncthreads();
         if (t < 64) {                    // lane L: bytes 255 - 4 L .. 252 - 4 L, in falling order
             u64 own = 0;
+#pragma unroll 1
             for (int e = 0; e < 4; ++e) own += s.whist[255 - 4 * t - e];
             u64 at = wave_scan(own) - own;
+#pragma unroll 1
             for (int e = 0; e < 4; ++e) {
                 const int byte = 255 - 4 * t - e;
                 const u64 h = s.whist[byte];
@@ -506,7 +494,7 @@ __device__ void cut(Shared &s, const Src &src, u64 need, In in, uint32_t *tkey, 
         prefix = s.prefix, left = s.need, mask |= 255u << shift;
         __syncthreads();
     }
-    if (WEIGHTS) {                       // one of the equal keys knows their weight
+    if (weights) {                       // one of the equal keys knows their weight
         src.each([&](uint32_t k, int, auto weight) {
             if (k == prefix && in(k)) s.before = weight();
         });
@@ -522,46 +510,12 @@ struct Kept {                            // keys above tkey, and the first `ties
     u64 ties, wt, wmin;
 };
 
-// top-p among what top-k left: moves k's threshold.
-template <typename Src>
-__device__ void cut_p(Shared &s, const Src &src, Bins bins, float top_p, Kept &k) {
-    const int t = threadIdx.x;
-    s.whist[2 * t] = s.whist[2 * t + 1] = 0;
-    __syncthreads();
-    src.each([&](uint32_t x, int, auto weight) {
-        if (x > k.tkey) {
-            const uint32_t b = bins.of_key(x);
-            if (b < BINS) {
-                const u64 w = weight();
-                if (w) atomicAdd(&s.whist[b], w);
-            }
-        }
-    });
-    if (t == 0 && k.tkey) {
-        const u64 w = k.ties * k.wt;
-        const uint32_t b = bins.of_key(k.tkey);
-        if (w && b < BINS) atomicAdd(&s.whist[b], w);
-    }
-    __syncthreads();
-    u64 need = 0, before;
-    uint32_t bin;
-    const u64 v[2] = {s.whist[2 * t], s.whist[2 * t + 1]};
-    scan_bins<2, S_THREADS>(v, s.wsum, s.found, [&](u64 sum) { return need = share(top_p, sum); }, &bin, &before);
-    const uint32_t low = k.tkey;
-    cut<true>(s, src, need - before, [&](uint32_t x) { return x >= low && bins.of_key(x) == bin; }, &k.tkey, &k.ties);
-}
-
-// Where src is a part of the row: the kept weights above the threshold and the keys equal to it in front of it, and the target that is in it.
-struct Start {
-    u64 sum, equal, target;
-};
-
 // The kept weights in the order of the indexes: each wave's sum over its stretch, then the wave whose stretch holds the target looks for it.
 template <typename Src>
-__device__ void pick(Shared &s, const Src &src, const Kept &k, float u, int32_t *token, const Start *start = nullptr) {
+__device__ void pick(Shared &s, const Src &src, const Kept &k, float u, int32_t *token) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const bool tied = k.tkey && k.wt >= k.wmin;
-    u64 above = 0, run = 0, seen = 0, total = start ? start->sum : 0, count = start ? start->equal : 0;
+    u64 above = 0, run = 0, seen = 0, total = 0, count = 0;
     uint32_t equal = 0;
     src.each([&](uint32_t x, int, auto weight) {
         if (x > k.tkey) {
@@ -572,13 +526,14 @@ __device__ void pick(Shared &s, const Src &src, const Kept &k, float u, int32_t 
     above = wave_sum(above), equal = wave_sum(equal);
     if (lane == 0) s.wsum[wave] = above, s.wcount[wave] = equal;
     __syncthreads();
+#pragma unroll 4
     for (int w = 0; w < WAVES; ++w) {
         if (w == wave) run = total, seen = count;
         total += s.wsum[w], count += s.wcount[w];
     }
     run += min(seen, k.ties) * k.wt;
     total += min(count, k.ties) * k.wt;
-    const u64 target = start ? start->target : target_of(u, total);
+    const u64 target = target_of(u, total);
     if (run > target || target >= run + above + (min(seen + equal, k.ties) - min(seen, k.ties)) * k.wt) return;
     uint32_t next = src.i0 + lane < src.i1 ? src.key(src.i0 + lane) : 0;
 #pragma unroll 1
@@ -594,6 +549,45 @@ __device__ void pick(Shared &s, const Src &src, const Kept &k, float u, int32_t 
         if (pos <= target && target < pos + w) *token = src.index(i + lane);
         run += __shfl(incl, 63), seen += __popcll(eqs);
         if (target < run) return;
+    }
+}
+
+// The same in a part of a row that is known to hold the target: `run` is what is kept above the threshold in front of it, `seen` the keys equal to it.  Each
+// thread has four, eight or sixteen consecutive logits; the one that finds the target among its own walks them.
+template <typename T>
+__device__ void pick_part(Shared &s, const Row<T> &r, const Weigher &weigh, int i0, int len, const Kept &k, u64 run, u64 seen, u64 target, int32_t *token) {
+    const int t = threadIdx.x, wave = t >> 6, per = len / S_THREADS, first = i0 + t * per, end = min(i0 + len, r.n);
+    const bool tied = k.tkey && k.wt >= k.wmin;
+    u64 above = 0;
+    uint32_t equal = 0;
+    auto weight = [&](float y) {
+        const u64 w = weigh.of(y);
+        return key_of(y) > k.tkey && w >= k.wmin ? w : 0;
+    };
+#pragma unroll 1
+    for (int i = first; i < first + per; i += 4) {
+        const f32x4 y = r.four(min(i, end));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) above += weight(y[e]), equal += tied && key_of(y[e]) == k.tkey;
+    }
+    const u64 sums = wave_scan(above);
+    const uint32_t eqs = wave_scan(equal);
+    if ((t & 63) == 63) s.wsum[wave] = sums, s.wcount[wave] = eqs;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) run += s.wsum[w], seen += s.wcount[w];
+    run += sums - above, seen += eqs - equal;
+    u64 at = run + min(seen, k.ties) * k.wt;
+    if (at > target || target >= run + above + min(seen + equal, k.ties) * k.wt) return;
+#pragma unroll 1
+    for (int i = first; i < first + per; i += 4) {
+        const f32x4 y = r.four(min(i, end));
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            u64 w = weight(y[e]);
+            if (tied && key_of(y[e]) == k.tkey) w = seen++ < k.ties ? k.wt : 0;
+            if (at <= target && target < at + w) *token = i + e;
+            at += w;
+        }
     }
 }
 
@@ -663,7 +657,7 @@ __global__ __launch_bounds__(S_THREADS) void sample_draw_k(SampleArgs a, PowerTa
     __syncthreads();
 
     // all parts' candidates, if they fit; lane p of each wave knows part p (there are 64 at most)
-    const bool by_sums = !set.top_k, cuts = set.top_k || set.top_p < 1;
+    const bool cuts = set.top_k || set.top_p < 1;
     const int held = cuts && lane < parts ? (int)w.part[lane].held : 0, past = wave_scan(held), n = __shfl(past, 63);
     const bool fits = !__any(held > P_CAP) && n <= CAP;
     if (fits)
@@ -677,77 +671,70 @@ __global__ __launch_bounds__(S_THREADS) void sample_draw_k(SampleArgs a, PowerTa
         }
     __syncthreads();
 
-    // The parts' sums are known but for what of the lists is kept: the part that holds the target, then the token in it.
-    auto pick_part = [&]() {
-        const bool tied = k.tkey && k.wt >= k.wmin;
-        if (t < 64) s.lw[t] = t < parts ? w.part[t].sum : 0, s.lidx[t] = 0;
-        __syncthreads();
-        for (int i = t; cuts && i < n; i += S_THREADS) {
-            const uint32_t key = s.key[i], at = s.idx[i] / (uint32_t)part_len;
-            const u64 x = s.weight[i];
-            if (key > k.tkey && x >= k.wmin) atomicAdd(&s.lw[at], x);
-            if (tied && key == k.tkey) atomicAdd(&s.lidx[at], 1u);
-        }
-        __syncthreads();
-        const u64 sum = s.lw[lane];
-        const uint32_t eq = s.lidx[lane];
-        const u64 sums = wave_scan(sum), before = sums - sum;
-        const uint32_t eqs = wave_scan(eq);
-        const u64 run = before + min((u64)(eqs - eq), k.ties) * k.wt, end = sums + min((u64)eqs, k.ties) * k.wt;
-        const u64 target = target_of(u, __shfl(end, 63));
-        const unsigned long long has = __ballot(run <= target && target < end);
-        const int part = __builtin_ctzll(has);
-        const Start start{__shfl(before, part), (u64)__shfl(eqs - eq, part), target};
-        pick(s, Whole<T>(r, weigh, part * part_len, min((part + 1) * part_len, r.n)), k, u, token, &start);
-    };
-    if (!cuts) return pick_part();
-
     // The bin that holds the cut.
-    u64 v[2], before = 0, need = 0;
-    uint32_t bin = 0;
-    if (set.few || !fits) {                  // (few: of the candidates that there are)
-        s.whist[2 * t] = s.whist[2 * t + 1] = 0;
-        __syncthreads();
-        auto count = [&](uint32_t x, int, auto weight) {
-            const uint32_t b = bins.of_key(x);
-            if (b >= BINS) return;
-            const u64 y = set.top_k ? 1 : weight();
-            if (y) atomicAdd(&s.whist[b], y);
-        };
-        if (fits) List(s, n).each(count);
-        else Whole<T>(r, weigh, 0, r.n).each(count);
-        __syncthreads();
-        v[0] = s.whist[2 * t], v[1] = s.whist[2 * t + 1];
-    } else v[0] = w.hist[2 * t], v[1] = w.hist[2 * t + 1];
-    const u64 total = scan_bins<2, S_THREADS>(v, s.wsum, s.found, [&](u64 sum) { return need = set.top_k ? (u64)set.top_k : share(set.top_p, sum); }, &bin, &before);
-    if (set.few && fits) {
-        if (t == 0) s.n = 0;
-        __syncthreads();
-        for (int i = t; i < n; i += S_THREADS)
-            if (bins.of_key(s.key[i]) <= bin) {
-                const uint32_t at = atomicAdd(&s.n, 1u);
-                if (at < SHORT) s.lkey[at] = s.key[i], s.lidx[at] = s.idx[i], s.lw[at] = s.weight[i];
+    const Source<T> src(s, r, weigh, fits, fits ? n : r.n);
+    u64 before = 0, need = 0, total = 0;
+    uint32_t bin = 0, low = 0;
+    bool weights = !set.top_k, counted = !set.few && fits;             // (few: of the candidates that there are)
+#pragma unroll 1
+    for (bool more = cuts; more;) {
+        if (!counted) {
+            s.whist[2 * t] = s.whist[2 * t + 1] = 0;
+            __syncthreads();
+            src.each([&](uint32_t x, int, auto weight) {
+                const uint32_t at = bins.of_key(x);
+                if (x <= k.tkey || at >= BINS) return;
+                const u64 y = weights ? weight() : 1;
+                if (y) atomicAdd(&s.whist[at], y);
+            });
+            if (t == 0 && k.tkey) {
+                const u64 y = k.ties * k.wt;
+                const uint32_t at = bins.of_key(k.tkey);
+                if (y && at < BINS) atomicAdd(&s.whist[at], y);
             }
-        __syncthreads();
-        const int m = s.n;
-        if (m <= SHORT) return draw_short(s, m, min(set.top_k, m), set.top_p, set.wmin, u, token);
-        __syncthreads();
-    }
-    auto rest = [&](const auto &src) {
-        auto in = [&](uint32_t x) { return bins.of_key(x) == bin; };
-        // top_k beyond all that has a weight cuts nothing
-        if (!set.top_k) cut<true>(s, src, need - before, in, &k.tkey, &k.ties);
-        else if (need <= total) cut<false>(s, src, need - before, in, &k.tkey, &k.ties);
-        k.wt = weigh.of_key(k.tkey);
-        if (set.top_k && set.top_p < 1) {
-            cut_p(s, src, bins, set.top_p, k);
+            __syncthreads();
+        }
+        const u64 v[2] = {counted ? w.hist[2 * t] : s.whist[2 * t], counted ? w.hist[2 * t + 1] : s.whist[2 * t + 1]};
+        total = scan_bins<2, S_THREADS>(v, s.wsum, s.found, [&](u64 sum) { return need = weights ? share(set.top_p, sum) : (u64)set.top_k; }, &bin, &before);
+        if (set.few && fits && !weights) {
+            if (t == 0) s.n = 0;
+            __syncthreads();
+            for (int i = t; i < n; i += S_THREADS)
+                if (bins.of_key(s.key[i]) <= bin) {
+                    const uint32_t at = atomicAdd(&s.n, 1u);
+                    if (at < SHORT) s.lkey[at] = s.key[i], s.lidx[at] = s.idx[i], s.lw[at] = s.weight[i];
+                }
+            __syncthreads();
+            const int m = s.n;
+            if (m <= SHORT) return draw_short(s, m, min(set.top_k, m), set.top_p, set.wmin, u, token);
+            __syncthreads();
+        }
+        if (weights || need <= total) {      // (a top_k beyond all that has a weight cuts nothing)
+            cut(s, src, weights, need - before, [&](uint32_t x) { return x >= low && bins.of_key(x) == bin; }, &k.tkey, &k.ties);
             k.wt = weigh.of_key(k.tkey);
         }
-        if (by_sums && fits) pick_part();
-        else pick(s, src, k, u, token);
-    };
-    if (fits) rest(List(s, n));
-    else rest(Whole<T>(r, weigh, 0, r.n));
+        more = !weights && set.top_p < 1;    // then top_p among what top_k left
+        weights = true, counted = false, low = k.tkey;
+    }
+    if (set.top_k || !fits) return pick(s, src, k, u, token);
+
+    // The parts' sums are known but for what of the lists is kept: the part that holds the target, then the token in it.
+    const bool tied = k.tkey && k.wt >= k.wmin;
+    if (t < 64) s.lw[t] = t < parts ? w.part[t].sum : 0, s.lidx[t] = 0;
+    __syncthreads();
+    for (int i = t; cuts && i < n; i += S_THREADS) {
+        const uint32_t key = s.key[i], at = s.idx[i] / (uint32_t)part_len;
+        const u64 x = s.weight[i];
+        if (key > k.tkey && x >= k.wmin) atomicAdd(&s.lw[at], x);
+        if (tied && key == k.tkey) atomicAdd(&s.lidx[at], 1u);
+    }
+    __syncthreads();
+    const u64 sum = s.lw[lane], sums = wave_scan(sum), front = sums - sum;
+    const uint32_t eq = s.lidx[lane], eqs = wave_scan(eq);
+    const u64 run = front + min((u64)(eqs - eq), k.ties) * k.wt, end = sums + min((u64)eqs, k.ties) * k.wt;
+    const u64 target = target_of(u, __shfl(end, 63));
+    const int part = __builtin_ctzll(__ballot(run <= target && target < end));
+    pick_part(s, r, weigh, part * part_len, part_len, k, __shfl(front, part), (u64)__shfl(eqs - eq, part), target, token);
 }
 
 constexpr int MAX_ROWS = 2048;               // of a launch
