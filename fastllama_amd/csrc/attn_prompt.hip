@@ -423,13 +423,13 @@ static hipError_t prompt_launch(const AttnArgs &a, int parts, hipStream_t st) {
 // (256, one for each CU) 61 -> 68.
 // Very few, behind many keys: the keys too are cut into parts of four tiles or more, until each CU has two workgroups, and joined by a second launch.  64
 // rows behind 30000, 32/8 heads of 128 in bf16: 575 -> 79 us (105 at one workgroup a CU); 16 behind 2000 in f16: 47 -> 20 (25 with parts of eight
-// tiles); 200 behind 1600, 8 heads in f32: 249 -> 44.  Not where each CU nearly has one anyway: 512 behind 1536, 32/32
-// in f16 (256 blocks), would take 46 instead of 42, 512 behind none 23 instead of 16.
+// tiles); 200 behind 1600, 8 heads in f32: 249 -> 44.  Where nearly each CU has one anyway, from 32 tiles on: 512 rows against 8192 keys, 32/32 in f16 (256
+// blocks), 168 -> 119, 4096 88 -> 71, 2048 49 -> 45; 1536 39 -> 40, 512 of a longer table 18 -> 24.  Three or four parts there, against 8192: 145, 122.
 static bool few_blocks(int type, int64_t rows, int64_t n_head_kv, int n_seq) { return type != FL_TYPE_F32 && (rows / 128 + n_seq) * n_head_kv < 512; }
 static int prompt_parts(int type, int64_t rows, int64_t n_head_kv, int n_seq, int64_t max_keys) {
     const int tile = type == FL_TYPE_F32 ? 32 : 64, block = few_blocks(type, rows, n_head_kv, n_seq) ? 64 : 128;
     const int64_t blocks = max((rows + block - 1) / block, (int64_t)n_seq) * n_head_kv;
-    if (blocks > 192) return 1;
+    if (blocks > 192 && max_keys < 32 * tile) return 1;
     return (int)max((int64_t)1, min(min((int64_t)16, 512 / max(blocks, (int64_t)1)), max_keys / (4 * tile)));
 }
 size_t attn_prompt_workspace(int type, int n_q, int n_seq, int n_head, int n_head_kv, int head_dim, int64_t max_keys) {

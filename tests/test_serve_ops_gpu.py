@@ -131,6 +131,12 @@ def test_prompt_few_rows_behind_many_keys(ops, T, H, Hkv, lq, lk, pages):
 
 
 @pytest.mark.parametrize("T", TYPES)
+@pytest.mark.parametrize("lk", [1100, 4300])
+def test_prompt_a_workgroup_for_each_cu_behind_many_keys(ops, T, lk):
+    check_prompt(ops, T, 28, 28, 64, [460 if T != F32 else 900], [lk], seed=lk, pages=64)
+
+
+@pytest.mark.parametrize("T", TYPES)
 def test_prompt_not_finite_behind_many_keys(ops, T):
     """As above for keys cut into parts: the last row's last key holds a value that is not finite, the rows before it do not see it."""
     q, k, v = randn(1, 4, 2, 64, dtype=T), randn(2, 4000, 1, 64, dtype=T), randn(3, 4000, 1, 64, dtype=T)
