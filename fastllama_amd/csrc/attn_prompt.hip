@@ -376,10 +376,11 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a, int parts
         }
 }
 
-// The rows whose keys were cut into parts: the same blocks, four rows at a time, 64 threads for a row.
+// The rows whose keys were cut into parts: the same blocks, a thread for four features of a row.
 template <typename T, int DP, bool PAGED, int ROWS>
 __global__ __launch_bounds__(256) void attn_prompt_join_k(AttnArgs a, int parts) {
-    const int n_head_kv = a.n_head / a.group, hk = blockIdx.x % n_head_kv, lane = threadIdx.x & 63, D = a.head_dim;
+    constexpr int LANES = DP / 4, SIDE = 256 / LANES;
+    const int n_head_kv = a.n_head / a.group, hk = blockIdx.x % n_head_kv, c = threadIdx.x % LANES * 4;
     const Block at = find_block<PAGED, ROWS>(a, blockIdx.x / n_head_kv, gridDim.x / n_head_kv);
     if (at.b < 0) return;
     const int rows = at.lq * a.group, r0 = at.blk * ROWS, past = at.lk - at.lq;
@@ -387,22 +388,22 @@ __global__ __launch_bounds__(256) void attn_prompt_join_k(AttnArgs a, int parts)
     int t0, t1;
     const int used = cut_tiles<Tile<T>::KT>(end, parts, 0, &t0, &t1);
     if (used == 1) return;
-    for (int row = r0 + blockIdx.y * 4 + (threadIdx.x >> 6); row < min(r0 + ROWS, rows); row += 4 * gridDim.y) {
+    for (int row = r0 + blockIdx.y * SIDE + threadIdx.x / LANES; row < min(r0 + ROWS, rows); row += SIDE * gridDim.y) {
         const int tok = row / a.group, head = hk * a.group + row % a.group;
         const float *part = (const float *)a.ws + ((int64_t)(at.q0 + tok) * a.n_head + head) * parts * (DP + 4);
-        float M = -INFINITY, l = 0, sum[2] = {0, 0};
+        float M = -INFINITY, l = 0;
+        f32x4 sum = {0, 0, 0, 0};
+#pragma unroll 4
         for (int s = 0; s < used; ++s) M = fmaxf(M, part[s * (DP + 4) + DP]);
 #pragma unroll 4
         for (int s = 0; s < used; ++s) {
             const float *p = part + s * (DP + 4);
-            const float m = p[DP], ls = p[DP + 1], x = p[min(lane, DP - 1)], y = p[min(lane + 64, DP - 1)];
-            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-            l += f == 0 ? 0.f : ls * f, sum[0] += f == 0 ? 0.f : x * f, sum[1] += f == 0 ? 0.f : y * f;
+            const f32x4 x = *(const f32x4 *)(p + c);
+            const float m = p[DP], ls = p[DP + 1], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+            if (f != 0) l += ls * f, sum += x * f;
         }
-        T *out = (T *)a.out + (int64_t)(at.q0 + tok) * a.o_ld + head * a.o_hs;
-        const float inv = l == 0 ? 0.f : 1 / l;
-        if (lane < D) out[lane] = (T)(sum[0] * inv);
-        if (lane + 64 < D) out[lane + 64] = (T)(sum[1] * inv);
+        typedef T x4 __attribute__((ext_vector_type(4)));
+        if (c < a.head_dim) *(x4 *)((T *)a.out + (int64_t)(at.q0 + tok) * a.o_ld + head * a.o_hs + c) = __builtin_convertvector(sum * (l == 0 ? 0.f : 1 / l), x4);
     }
 }
 
@@ -412,7 +413,7 @@ static hipError_t prompt_launch(const AttnArgs &a, int parts, hipStream_t st) {
     const int64_t rows = (int64_t)a.n_q * a.group, blocks = (rows / ROWS + a.n_seq) * (a.n_head / a.group);   // every sequence may end inside a block
     if (blocks > INT32_MAX) return hipErrorInvalidValue;
     attn_prompt_k<T, DP, PAGED, KS, W><<<dim3((unsigned)blocks, parts), 64 * W, 0, st>>>(a, parts);
-    if (parts > 1) attn_prompt_join_k<T, DP, PAGED, ROWS><<<dim3((unsigned)blocks, 8), 256, 0, st>>>(a, parts);
+    if (parts > 1) attn_prompt_join_k<T, DP, PAGED, ROWS><<<dim3((unsigned)blocks, ROWS * DP / 1024), 256, 0, st>>>(a, parts);
     return hipGetLastError();
 }
 
