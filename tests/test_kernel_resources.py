@@ -1,0 +1,48 @@
+"""CPU: what the compiler gave the kernels of the built library, read from the metadata of its gfx950 code objects (compiled from this tree's sources)."""
+import os
+import re
+import struct
+import subprocess
+
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+LIB = os.path.join(ROOT, "fastllama_amd", "libfastllama_hip.so")
+READELF = os.path.join(os.environ.get("ROCM_PATH", "/opt/rocm"), "llvm", "bin", "llvm-readelf")
+
+
+def code_objects(data):
+    """The ELF images for AMD GPUs (machine 224) inside the library, from header to the end of their section table."""
+    at = data.find(b"\x7fELF", 1)
+    while at >= 0:
+        if struct.unpack_from("<H", data, at + 18)[0] == 224:
+            table, = struct.unpack_from("<Q", data, at + 40)
+            size, count = struct.unpack_from("<HH", data, at + 58)
+            yield data[at:at + table + size * count]
+        at = data.find(b"\x7fELF", at + 4)
+
+
+@pytest.fixture(scope="module")
+def scratch(tmp_path_factory):
+    """{demangled kernel: bytes of scratch a lane}"""
+    if not os.path.exists(READELF):
+        pytest.skip("llvm-readelf is not installed")
+    if not os.path.exists(LIB):
+        subprocess.check_call([os.path.join(ROOT, "build.sh")])
+    found, file = {}, tmp_path_factory.mktemp("code") / "object"
+    for image in code_objects(open(LIB, "rb").read()):
+        file.write_bytes(image)
+        notes = subprocess.run([READELF, "--notes", str(file)], capture_output=True, text=True, check=True).stdout
+        for kernel in re.split(r"^  - ", notes.split("amdhsa.kernels:")[-1], flags=re.M)[1:]:
+            name, size = re.search(r"\.name:\s+(\S+)", re.sub(r"^ {8,}.*\n", "", kernel, flags=re.M)), re.search(r"\.private_segment_fixed_size:\s+(\d+)", kernel)
+            if name and size:
+                found[name.group(1)] = int(size.group(1))
+    names = subprocess.run(["c++filt"], input="\n".join(found), capture_output=True, text=True, check=True).stdout.split("\n")
+    return dict(zip(names, found.values()))
+
+
+def test_streaming_decode_kernels_keep_their_registers(scratch):
+    """The one-wave-per-row-group kernel of a decode step has its weights in flight in registers: one that spills waits for scratch memory in its loop."""
+    kernels = {k: v for k, v in scratch.items() if "gemv1_q4_exact_stream_kernel" in k}
+    assert len(kernels) >= 30
+    assert not {k: v for k, v in kernels.items() if v}
