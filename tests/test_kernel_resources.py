@@ -46,3 +46,12 @@ def test_streaming_decode_kernels_keep_their_registers(scratch):
     kernels = {k: v for k, v in scratch.items() if "gemv1_q4_exact_stream_kernel" in k}
     assert len(kernels) >= 30
     assert not {k: v for k, v in kernels.items() if v}
+
+
+@pytest.mark.parametrize("kernel", ["attn_prompt_k", "attn_prompt_join_k", "attn_decode_k", "attn_join_k", "kv_append_k", "sample_scan_k", "sample_hist_k", "sample_gather_k",
+                                    "sample_draw_k"])
+def test_operators_over_several_sequences_use_no_scratch(scratch, kernel):
+    """Their entry points allocate nothing, so no launch of theirs may make the runtime allocate scratch memory."""
+    kernels = {k: v for k, v in scratch.items() if kernel in k}
+    assert len(kernels) >= 3
+    assert not {k: v for k, v in kernels.items() if v}
