@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, i
 #pragma unroll
             for (int d = 0; d < DB; ++d) o[d] *= f;
         }
-        const float ref = m == -INFINITY ? 0.f : m;
+        const float ref = (m == -INFINITY ? 0.f : m) - P_SHIFT<T>;
         xp p;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, i
             for (int r = 0; r < 4; ++r) {
                 const float e = __builtin_amdgcn_exp2f(fmaf(s[kb][r], a.scale_log2, -ref));
                 l += e;
-                p[4 * kb + r] = (T)e;
+                p[4 * kb + r] = (T)e;                                  // (rounded for the second product, as in attn_prompt.hip)
             }
 #pragma unroll
         for (int d = 0; d < DB; ++d) {

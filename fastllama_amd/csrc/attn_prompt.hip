@@ -11,8 +11,9 @@
 // columns are query rows again: the rescaling factor is a lane's own.  V^T comes out of LDS by transposing reads.
 //
 // The softmax's reference is not the running maximum but a value at most 2^8 below it: the accumulators are rescaled only when the maximum
-// has moved by more (p <= 2^8 fits f16 and costs no precision).  p is rounded to the inputs' type for the second product (the error of a
-// weighted mean of values that are themselves of that type); scores, sums and outputs are f32 until the one rounding at the end.
+// has moved by more.  p is rounded to the inputs' type for the second product (the error of a weighted mean of values that are themselves of that
+// type); scores, sums and outputs are f32 until the one rounding at the end.  f16 has p only down to 2^-24, so there it is taken 2^P_SHIFT times as large,
+// which cancels against the sum: p <= 2^15 still fits, and what is lost of a key is at most 2^-32 of the largest weight.
 #include "serve_kernels.h"
 #include "serve_device.h"
 #include "../../include/fastllama_hip.h"
@@ -296,7 +297,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a, int parts
 #pragma unroll
                 for (int d = 0; d < DB; ++d) o[d] *= f;
             }
-            const float ref = m == -INFINITY ? 0.f : m;
+            const float ref = (m == -INFINITY ? 0.f : m) - P_SHIFT<T>;
             x8 p[KB][2];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)

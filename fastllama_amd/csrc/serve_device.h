@@ -56,6 +56,12 @@ __device__ inline float sum_halves(float x) {
     return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
 
+// Numerators of the softmax are 2^P_SHIFT as large in f16, whose smallest is 2^-24 (attn_prompt.hip).
+template <typename T>
+constexpr float P_SHIFT = 0.f;
+template <>
+inline constexpr float P_SHIFT<h16> = 7.f;
+
 typedef __attribute__((address_space(3))) s16x4 *lds_s16x4;
 
 template <typename T>

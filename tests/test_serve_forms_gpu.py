@@ -125,3 +125,35 @@ def test_absent_pages_on_both_sides_of_the_range(ops, T, D, page):
             kb, vb = (torch.cat([x[a:a + n][there[b]], torch.full((rest, Hkv, D), y, dtype=T, device="cuda")]) for x, y in ((k, 0.25), (v, 0.5)))
             near(got[b:b + 1], *attention64(q[b:b + 1], kb, vb, D ** -0.5), (b, cu is None))
             a += n
+
+
+# ------------------------------------------------------------------------------------------------ weights that f16 can hardly hold
+def sinks(seed, rows, keys, H, Hkv, gap):
+    """Every 32nd key outweighs the others by e^gap and has the value 0: what comes out is the others' share."""
+    q, k, v = (torch.zeros(n, h, 64, device="cuda") for n, h in ((rows, H), (keys, Hkv), (keys, Hkv)))
+    q[:, :, 0] = 1
+    k[:, :, 0] = 0.05 * randn(seed, keys, Hkv)
+    v += 256 + 16 * randn(seed + 1, keys, Hkv, 64)
+    k[::32, :, 0], v[::32] = gap, 0
+    return q.half(), k.half(), v.half()
+
+
+@pytest.mark.parametrize("gap", [14.0, 18.0])
+@pytest.mark.parametrize("rows,keys,H,Hkv,pages", [(1, 200, 2, 2, 16), (1, 5000, 4, 2, 64), (3, 5000, 2, 1, 0), (40, 300, 2, 2, 16), (300, 400, 128, 128, 0), (300, 400, 128, 128, 64)])
+def test_small_weights_beside_large_ones_in_f16(ops, rows, keys, H, Hkv, pages, gap):
+    """As attention64's bound, but for its term for p below f16's range: p is held as 2^7 p, its smallest step 2^-24, so half a step of it is 2^-32 (of a sum
+    of 1 or more)."""
+    q, k, v = sinks(1, rows, keys, H, Hkv, gap)
+    want, bound = attention64(q, k, v, 1.0)
+    s = torch.matmul(q.double().transpose(0, 1), k.double().repeat_interleave(H // Hkv, 1).permute(1, 2, 0).contiguous())
+    seen = torch.arange(keys, device="cuda")[None, :] <= torch.arange(rows, device="cuda")[:, None] + (keys - rows)
+    l = torch.where(seen, torch.exp(s - s.amax(-1, keepdim=True)), 0.0).sum(-1, keepdim=True)
+    total = (seen.double() @ v.double().abs().repeat_interleave(H // Hkv, 1).transpose(0, 1).contiguous() / l).transpose(0, 1)
+    bound = bound + (2.0 ** -32 - 2.0 ** -25) * total
+    assert (bound < 0.1 * want).all()
+    if pages:
+        cache, table = scatter(ops, k, v, [keys], pages, 1)
+        for cu in ([None] if rows == 1 else []) + [i32([0, rows])]:
+            near(ops.attn_pages(q, cache, table, i32([keys]), cu, 1.0), want, bound)
+    else:
+        near(ops.attn_prompt(q, k, v, i32([0, rows]), i32([0, keys]), 1.0), want, bound)
