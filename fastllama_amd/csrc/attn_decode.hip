@@ -201,7 +201,7 @@ __global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, i
     __syncthreads();
     float M = ms[0][n];
     for (int w = 1; w < DEC_WAVES; ++w) M = fmaxf(M, ms[w][n]);
-    const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
+    const float f = factor(m, M);
     float *mine = (float *)vs[wave];
 #pragma unroll
     for (int d = 0; d < DB; ++d)
@@ -213,7 +213,7 @@ __global__ __launch_bounds__(64 * DEC_WAVES, 2) void attn_decode_k(AttnArgs a, i
         float mq = ms[0][q], lq = 0, sum = 0;
         for (int w = 1; w < DEC_WAVES; ++w) mq = fmaxf(mq, ms[w][q]);
         for (int w = 0; w < DEC_WAVES; ++w) {
-            lq += ms[w][q] == -INFINITY ? 0.f : ls[w][q] * __builtin_amdgcn_exp2f(ms[w][q] - mq);
+            lq += ls[w][q] * factor(ms[w][q], mq);
             sum += ((const float *)vs[w])[e];
         }
         const int head = head0 + q;
@@ -249,8 +249,8 @@ __global__ __launch_bounds__(128 * GROUPS) void attn_join_k(AttnArgs a, int chun
     for (int s = g; s < n; s += GROUPS) {
         const float *p = part + (int64_t)s * (D + 2);
         const float x = p[dd], m = p[D], ls = p[D + 1];
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-        l += f == 0 ? 0.f : ls * f, sum += f == 0 ? 0.f : x * f;
+        const float f = factor(m, M);
+        l += ls * f, sum += x * f;
     }
     acc[g][d] = sum;
     if (d == 0) den[g] = l;

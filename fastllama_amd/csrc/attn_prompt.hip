@@ -329,7 +329,7 @@ __global__ __launch_bounds__(64 * W, 2) void attn_prompt_k(AttnArgs a, int parts
         __syncthreads();
         if (kb0) return;
         const float m2 = part[16 * DB * 64], l2 = part[(16 * DB + 1) * 64], M = fmaxf(m, m2);
-        const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M), f2 = m2 == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m2 - M);
+        const float f = factor(m, M), f2 = factor(m2, M);
         l = l * f + l2 * f2, m = M;
 #pragma unroll
         for (int d = 0; d < DB; ++d)
@@ -403,8 +403,8 @@ __global__ __launch_bounds__(256) void attn_prompt_join_k(AttnArgs a, int parts)
         for (int s = 0; s < used; ++s) {
             const float *p = part + s * (DP + 4);
             const f32x4 x = *(const f32x4 *)(p + c);
-            const float m = p[DP], ls = p[DP + 1], f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M);
-            if (f != 0) l += ls * f, sum += x * f;
+            const float ls = p[DP + 1], f = factor(p[DP], M);
+            l += ls * f, sum += x * f;
         }
         typedef T x4 __attribute__((ext_vector_type(4)));
         if (c < a.head_dim) *(x4 *)((T *)a.out + (int64_t)(at.q0 + tok) * a.o_ld + head * a.o_hs + c) = __builtin_convertvector(sum * (l == 0 ? 0.f : 1 / l), x4);

@@ -56,6 +56,10 @@ __device__ inline float sum_halves(float x) {
     return __uint_as_float(w[0]) + __uint_as_float(w[1]);
 }
 
+// What a part of a row's keys with the maximum m counts for beside the whole's, M.  A part without keys has m = -infinity and sums of 0, one whose scores
+// are all no numbers has the sum NaN with it: that stays NaN whatever it is multiplied by.
+__device__ inline float factor(float m, float M) { return m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - M); }
+
 // Numerators of the softmax are 2^P_SHIFT as large in f16, whose smallest is 2^-24 (attn_prompt.hip).
 template <typename T>
 constexpr float P_SHIFT = 0.f;

@@ -157,3 +157,42 @@ def test_small_weights_beside_large_ones_in_f16(ops, rows, keys, H, Hkv, pages, 
             near(ops.attn_pages(q, cache, table, i32([keys]), cu, 1.0), want, bound)
     else:
         near(ops.attn_prompt(q, k, v, i32([0, rows]), i32([0, keys]), 1.0), want, bound)
+
+
+# ------------------------------------------------------------------------------------------------ parts of a row that are joined
+@pytest.mark.parametrize("T", TYPES)
+@pytest.mark.parametrize("first,end", [(0, 4990), (1024, 2048), (0, 40), (2500, 2501)])
+@pytest.mark.parametrize("form", ["decode", "pages", "prompt", "short"])
+def test_keys_that_are_no_numbers_reach_the_rows_that_see_them(ops, T, first, end, form):
+    """NaN in the keys of one key head, also in all keys that one wave, chunk or part has: its query heads become NaN, the others are as without."""
+    keys, rows, H, Hkv, D = 5000 if form != "short" else 60, 1 if form == "decode" else 3, 4, 2, 64
+    q, k, v = randn(1, rows, H, D, dtype=T), randn(2, keys, Hkv, D, dtype=T), randn(3, keys, Hkv, D, dtype=T)
+    want, bound = attention64(q, k, v, D ** -0.5)
+    first, end = (first, end) if form != "short" else (min(first, 31), min(end, 58))
+    k[first:end, 0] = float("nan")
+    if form in ("decode", "pages"):
+        cache, table = scatter(ops, k, v, [keys], 64, 1)
+        got = ops.attn_pages(q, cache, table, i32([keys]), None if form == "decode" else i32([0, rows]))
+    else:
+        got = ops.attn_prompt(q, k, v, i32([0, rows]), i32([0, keys]))
+    assert got[:, :2].isnan().all()
+    near(got[:, 2:], want[:, 2:], bound[:, 2:])
+
+
+@pytest.mark.parametrize("T", TYPES)
+@pytest.mark.parametrize("form", ["decode", "pages", "prompt"])
+def test_an_infinite_value_of_no_weight_reaches_the_rows_that_see_it(ops, T, form):
+    """A stretch of keys far below all others, one of their values infinite: its feature is not finite, the others are as without."""
+    keys, rows, D = 5000, 1 if form == "decode" else 3, 64
+    q, k, v = torch.ones((rows, 2, D), dtype=T, device="cuda"), randn(2, keys, 1, D, dtype=T, scale=0.1), randn(3, keys, 1, D, dtype=T)
+    k[1024:2048] -= 25                                        # 64 * 25 / 8 = 200 below
+    want, bound = attention64(q, k, v, D ** -0.5)
+    v[1500, 0, 5] = float("inf")
+    if form == "prompt":
+        got = ops.attn_prompt(q, k, v, i32([0, rows]), i32([0, keys]))
+    else:
+        cache, table = scatter(ops, k, v, [keys], 64, 1)
+        got = ops.attn_pages(q, cache, table, i32([keys]), None if form == "decode" else i32([0, rows]))
+    assert not got[:, :, 5].isfinite().any()
+    rest = [d for d in range(D) if d != 5]
+    near(got[:, :, rest], want[:, :, rest], bound[:, :, rest])
