@@ -18,6 +18,7 @@
 //
 // Weights are whole numbers, w_i * 2^44 rounded once from a 64-bit exponential: their sums are exact and do not depend on the order of
 // additions or atomics, and 2^18 of them fit 63 bits.  A kept set is a threshold: all keys above `tkey` and the first `ties` that equal it.
+#include <cfloat>
 #include <cmath>
 #include "serve_kernels.h"
 #include "serve_device.h"
@@ -132,7 +133,7 @@ struct Settings {
 struct Bins {
     float half_max, per;                 // per > 0
     __device__ uint32_t operator()(float x) const { return (uint32_t)__builtin_amdgcn_fmed3f(fmaf(x, -0.5f, half_max) * per, 0.f, 2.f * BINS); }
-    __device__ Bins(float max, float temp) : half_max(0.5f * max), per(fmaxf(fminf(128.f / temp, 3e38f), 1e-30f)) {}
+    __device__ Bins(float max, float temp) : half_max(0.5f * max), per(fmaxf(fminf(128.f / temp, 3e38f), FLT_MIN)) {}   // (f32's whole range is 8 FLT_MIN steps)
     __device__ uint32_t of_key(uint32_t key) const { return (*this)(value_of(key)); }
 };
 

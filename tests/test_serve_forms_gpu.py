@@ -94,6 +94,24 @@ def test_sample_all_rows_one_large_top_k(ops):
         assert ops.sample(l, u.cuda(), 0.9, k, 0.95).tolist() == want, k
 
 
+@pytest.mark.parametrize("T", [F32, BF16])
+@pytest.mark.parametrize("V", [5, 5000])
+def test_sample_temperatures_of_the_largest_size(ops, T, V):
+    """Logits over all of the type's range, at temperatures beside which even their distances are small: each weighs something."""
+    settings = [(t, k, p, m) for t in (math.inf, 3e38, 1e37, 1e33, 1e31) for k, p, m in ((0, 1.0, 0.0), (2, 1.0, 0.0), (0, 0.5, 0.0), (300, 0.9, 0.0), (0, 1.0, 0.3))]
+    rows, rng = len(settings), np.random.default_rng(V)
+    l = torch.from_numpy(rng.uniform(-3.3e38, 3.3e38, (rows, V)).astype(np.float32)).cuda().to(T)
+    l[:, 1], l[:, 3] = -math.inf, torch.finfo(T).min
+    u = torch.from_numpy(rng.random(rows).astype(np.float32))
+    f = lambda i: torch.tensor([s[i] for s in settings], dtype=F32, device="cuda")
+    got = ops.sample(l, u.cuda(), f(0), f(1).int(), f(2), f(3)).tolist()
+    ln = l.double().cpu().numpy()
+
+    def want(x, u, t, *cuts):                                # (-infinity / infinity is no number; distances of 1e-21 weigh 1 in 64 bits as well)
+        return sample64(x * 1e-60, u, 1.0, *cuts) if t == math.inf else sample64(x, u, t, *cuts)
+    assert got == [want(ln[r], u[r].item(), *settings[r]) for r in range(rows)]
+
+
 # ------------------------------------------------------------------------------------------------ pages
 @pytest.mark.parametrize("T", TYPES)
 @pytest.mark.parametrize("D", [32, 64, 128])
