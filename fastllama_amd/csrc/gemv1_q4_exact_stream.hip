@@ -41,6 +41,9 @@ __device__ __forceinline__ float sq_bcast(float v) {      // value of lane (quad
     return dpp_f32<SRC | (SRC << 2) | (SRC << 4) | (SRC << 6)>(v);
 }
 
+// s_waitcnt for all but n vector-memory loads
+constexpr int vm_left(int n) { return (n & 15) | (n >> 4) << 14 | 7 << 4 | 15 << 8; }
+
 #ifdef LLC_TIMING   // development build only (scripts/dev/stream_timeline.py): per-workgroup wall-clock stamps of every launch since the last reset
 constexpr unsigned ST_TL_CAP = 1u << 16;
 constexpr int ST_TL_W = 12;       // int64 per record: entry, loads issued, prologue done, loop end of waves 0..3, chains reduced + stored, end, id, spare x2
@@ -80,6 +83,7 @@ __global__ __launch_bounds__(64 * MAXW, MAXW == 4 ? 2 : (MAXW == 8 && U == 8 && 
     const uint16_t *__restrict__ silu_tab, int8_t *__restrict__ oq, float *__restrict__ od, float *__restrict__ os,
     const TpTail *__restrict__ tt, const StreamPrefetch pf) {
     constexpr bool Q41 = TYPE == FL_TYPE_Q4_1;
+    constexpr bool HELPERS = (MAXW == 8 && U == 8) || MAXW == 16;                // forms with prologue-only waves
     constexpr int NT = 256;
     extern __shared__ __attribute__((aligned(16))) unsigned char gsm[];
     __shared__ double sh[4];
@@ -91,6 +95,7 @@ __global__ __launch_bounds__(64 * MAXW, MAXW == 4 ? 2 : (MAXW == 8 && U == 8 && 
     float *ld_ = reinterpret_cast<float *>(gsm + (size_t)NQP * 128);
     float *ls_ = ld_ + 4 * NQP;
 
+    const int pf_pos = EPI == 0 && PRO == 1 && pf.kc ? *pf.pos : 0;              // (a scalar load, as long as no wait stands in front of it)
     ST_DECL;
     ST_STAMP(0);
     GP_DECL(PRO);
@@ -154,13 +159,18 @@ __global__ __launch_bounds__(64 * MAXW, MAXW == 4 ? 2 : (MAXW == 8 && U == 8 && 
     //  profiles/r06_decode_exact.md: a short s_sleep between the activation's requests and the weights' (0.2 us: no change, 0.5 us: -2 %); the next quad's
     //  activation read from LDS one quad ahead (no change at 16 quads in flight, -8 % at 8); the two chains as one v_pk_fma_f32 with the lane sums
     //  converted by a v_dot4 onto the bits of 1.5 x 2^23 and a packed subtract (-22 % VALU instructions in the loop, bit-identical, no change in tok/s).)
-    if (active) {
+    // The waits on the activation's loads are written out, and no path leads round them: where one does (threads past 256, waves without a row group), the
+    // compiler has to take those loads as still on their way, and a register of theirs that the loop reuses makes it wait for EVERY load at the head of
+    // each round -- with packed f32 instructions the registers happened to fall otherwise.  7B Q4_0 1.576 -> 1.509 ms per token, Q4_1 1.881 -> 1.849.
+    if constexpr (PRO == 1 && HELPERS) __builtin_amdgcn_s_waitcnt(vm_left(0));        // (streaming waves have none; the others need them now)
+    if (active || (PRO == 1 && !HELPERS)) {                                           // (a wave without a row group: the last one's, for nothing)
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             req_scale(i, i);
             req_nib(i, i);
             __builtin_amdgcn_sched_barrier(0);
         }
+        if constexpr (PRO == 1 && !HELPERS) __builtin_amdgcn_s_waitcnt(vm_left((Q41 ? 3 : 2) * U));
     }
 
     // ---- the K / V history of the attention that follows: one dword per 128-byte line, for the heads of this workgroup's XCD class
@@ -169,7 +179,7 @@ __global__ __launch_bounds__(64 * MAXW, MAXW == 4 ? 2 : (MAXW == 8 && U == 8 && 
     float pf0 = 0.f, pf1 = 0.f;
     if constexpr (EPI == 0 && PRO == 1) {
         if (pf.kc) {
-            const int pos = min(*pf.pos, 256), cls = (int)blockIdx.x & 7, ncls_wg = ((int)gridDim.x + 7 - cls) >> 3;
+            const int pos = min(pf_pos, 256), cls = (int)blockIdx.x & 7, ncls_wg = ((int)gridDim.x + 7 - cls) >> 3;
             const int hpc = (pf.H + 7 - cls) >> 3;                            // heads h = cls, cls + 8, ...
             const int klines = pf.D >> 5, vlines = (pos + 31) >> 5;          // 128-byte lines per K row of a head / per V row's history
             // (K rows only: 618 / 394 tok/s at 7B / 13B against 619 / 397 with both and 617 / 385 without the hint, profiles/r06_decode_exact.md)
