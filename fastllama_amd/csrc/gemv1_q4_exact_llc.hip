@@ -368,27 +368,36 @@ __global__ __launch_bounds__(64 * NK, (!PERSIST && QPW <= 8 && NK == 4) ? 3 : 1)
                     while (__hip_atomic_load(&chain_seq[par], __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_WORKGROUP) < turn) __builtin_amdgcn_s_sleep(1);
                     a0 = accs[par][lane][0]; a1 = accs[par][lane][1]; if (Q41) summs = accs[par][lane][2];
                 }
+                auto link = [&](int i) __attribute__((always_inline)) {         // a quad's part of the chains
+                    float sxv[4] = {0.f, 0.f, 0.f, 0.f}, msb[4] = {0.f, 0.f, 0.f, 0.f};
+                    if constexpr (PRE_M) {
 #pragma unroll
-                for (int i = 0; i < QPW; ++i) {
-                    if (i < nq) {
-                        float sxv[4] = {0.f, 0.f, 0.f, 0.f}, msb[4] = {0.f, 0.f, 0.f, 0.f};
-                        if constexpr (PRE_M) {
-#pragma unroll
-                            for (int blk = 0; blk < 4; ++blk) { msb[blk] = msb_[i][blk]; sxv[blk] = sxv_[i][blk]; }
-                        } else if (Q41) {
-                            // (m_w of a block sits in one lane of the row's quad, as d_w does; broadcast here, in the chain -- kept as four registers
-                            //  per quad since the order-free part it cost Q4_1 its third workgroup per CU: round 5)
-                            msb[0] = quad_bcast<0>(mw[i]); msb[1] = quad_bcast<1>(mw[i]); msb[2] = quad_bcast<2>(mw[i]); msb[3] = quad_bcast<3>(mw[i]);
-                            const float4 sx4 = *reinterpret_cast<const float4 *>(ls_ + 4 * (qlo + i));
-                            sxv[0] = sx4.x; sxv[1] = sx4.y; sxv[2] = sx4.z; sxv[3] = sx4.w;
-                        }
-#pragma unroll
-                        for (int blk = 0; blk < 4; ++blk) {
-                            a0 = __fmaf_rn(dd[i][blk], f0[i][blk], a0);
-                            a1 = __fmaf_rn(dd[i][blk], f1[i][blk], a1);
-                            if (Q41) summs = __fmaf_rn(msb[blk], sxv[blk], summs);      // (a block past K: s_x = 0, m_w finite)
-                        }
+                        for (int blk = 0; blk < 4; ++blk) { msb[blk] = msb_[i][blk]; sxv[blk] = sxv_[i][blk]; }
+                    } else if (Q41) {
+                        // (m_w of a block sits in one lane of the row's quad, as d_w does; broadcast here, in the chain -- kept as four registers
+                        //  per quad since the order-free part it cost Q4_1 its third workgroup per CU: round 5)
+                        msb[0] = quad_bcast<0>(mw[i]); msb[1] = quad_bcast<1>(mw[i]); msb[2] = quad_bcast<2>(mw[i]); msb[3] = quad_bcast<3>(mw[i]);
+                        const float4 sx4 = *reinterpret_cast<const float4 *>(ls_ + 4 * (qlo + i));
+                        sxv[0] = sx4.x; sxv[1] = sx4.y; sxv[2] = sx4.z; sxv[3] = sx4.w;
                     }
+#pragma unroll
+                    for (int blk = 0; blk < 4; ++blk) {
+                        a0 = __fmaf_rn(dd[i][blk], f0[i][blk], a0);
+                        a1 = __fmaf_rn(dd[i][blk], f1[i][blk], a1);
+                        if (Q41) summs = __fmaf_rn(msb[blk], sxv[blk], summs);      // (a block past K: s_x = 0, m_w finite)
+                    }
+                };
+                // A slice that is full but for its last quad goes without a branch for each quad: all waves wait for the chain in front of theirs, and
+                // without packed f32 instructions the compiler laid those quads out as two branches each.  7B Q4_0 1.507 -> 1.456 ms per token, Q4_1
+                // 1.850 -> 1.810.
+                if (nq >= QPW - 1) {
+#pragma unroll
+                    for (int i = 0; i < QPW - 1; ++i) link(i);
+                    if (nq == QPW) link(QPW - 1);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < QPW - 2; ++i)
+                        if (i < nq) link(i);
                 }
                 if (k < NK - 1 || (PERSIST && pass < npass - 1)) { accs[par][lane][0] = a0; accs[par][lane][1] = a1; if (Q41) accs[par][lane][2] = summs; }
                 __hip_atomic_store(&chain_seq[par], turn + 1, __ATOMIC_RELEASE, __HIP_MEMORY_SCOPE_WORKGROUP);
