@@ -266,7 +266,7 @@ static hipError_t decode_launch(const AttnArgs &a, hipStream_t st) {
     const int n_head_kv = a.n_head / a.group, q_blocks = (a.group + 15) / 16;
     const int64_t max_len = (int64_t)a.n_table << a.page_shift, blocks = decode_blocks(a.n_seq, a.n_head, n_head_kv);
     const int chunk = decode_chunk(blocks, max_len, sizeof(T) == 4 ? 16 * DEC_WAVES : 32 * DEC_WAVES), splits = (int)((max_len + chunk - 1) / chunk);
-    if (blocks * splits > INT32_MAX || (int64_t)a.n_seq * a.n_head > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks * splits * 64 * DEC_WAVES > UINT32_MAX) return hipErrorInvalidValue;
     const dim3 g((unsigned)(blocks * splits));
     if (a.head_dim <= 32) attn_decode_k<T, 32><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);
     else if (a.head_dim <= 64) attn_decode_k<T, 64><<<g, 64 * DEC_WAVES, 0, st>>>(a, chunk, splits, q_blocks);

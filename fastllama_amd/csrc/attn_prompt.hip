@@ -415,7 +415,7 @@ template <typename T, int DP, bool PAGED, int KS, int W>
 static hipError_t prompt_launch(const AttnArgs &a, int parts, hipStream_t st) {
     constexpr int ROWS = 32 * W / KS;
     const int64_t rows = (int64_t)a.n_q * a.group, blocks = (rows / ROWS + a.n_seq) * (a.n_head / a.group);   // every sequence may end inside a block
-    if (blocks > INT32_MAX) return hipErrorInvalidValue;
+    if (blocks * 64 * W > UINT32_MAX) return hipErrorInvalidValue;
     attn_prompt_k<T, DP, PAGED, KS, W><<<dim3((unsigned)blocks, parts), 64 * W, 0, st>>>(a, parts);
     if (parts > 1) attn_prompt_join_k<T, DP, PAGED, ROWS><<<dim3((unsigned)blocks, ROWS * DP / 1024), 256, 0, st>>>(a, parts);
     return hipGetLastError();

@@ -43,7 +43,6 @@ __global__ __launch_bounds__(256) void kv_append_k(AppendArgs a) {
 
 hipError_t kv_append(const AppendArgs &a, int src_type, int type, hipStream_t st) {
     const int64_t n = (int64_t)a.n_tok * a.n_head_kv * (a.head_dim >> 3);
-    if ((n + 255) / 256 > INT32_MAX) return hipErrorInvalidValue;
     const dim3 g((unsigned)((n + 255) / 256));
     if (type == FL_TYPE_F32) kv_append_k<float, float><<<g, 256, 0, st>>>(a);
     else if (type == FL_TYPE_F16 && src_type == FL_TYPE_F32) kv_append_k<float, h16><<<g, 256, 0, st>>>(a);

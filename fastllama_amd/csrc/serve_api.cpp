@@ -28,6 +28,8 @@ static int check_dim(const char *fn, int type, int head_dim, int n_head_kv) {
 
 // Rows are read and written in 16-byte pieces, and 64 of them are within 32 bits of an address.
 constexpr int64_t MAX_ROW = 1 << 22;
+// Kernels count rows and keys in 32 bits, up to the end of a block (256 rows) or tile (64 keys) that the last one is in.
+constexpr int MAX_COUNT = INT32_MAX - 511;
 static int check_heads(const char *fn, const char *what, const fl_heads *h, int type, int rows) {
     if (!h || rows < 0) return set_error(FL_EINVAL, "%s: %s: null view or %d rows", fn, what, rows);
     if (rows == 0) return FL_OK;
@@ -79,6 +81,8 @@ int fl_kv_append(const fl_kv_pages *c, int src_type, const fl_heads *k, const fl
     if ((c->n_pages > 1 && !c->page_stride) || (c->n_head_kv > 1 && !c->head_stride) || !c->slot_stride) return set_error(FL_EINVAL, "%s: a stride of 0 in the cache", fn);
     if (n_tokens == 0) return FL_OK;
     FL_TRY(check_table(fn, c, table_dev, table_ld, n_table, n_seq));
+    if ((int64_t)n_tokens * c->n_head_kv * (c->head_dim / 8) > UINT32_MAX - 255)         // (a launch has fewer than 2^32 threads)
+        return set_error(FL_EINVAL, "%s: %d rows of %d heads of %d: more than 2^35 elements", fn, n_tokens, c->n_head_kv, c->head_dim);
     if (!n_past_dev || (!cu_dev && n_seq != n_tokens)) return set_error(FL_EINVAL, "%s: no n_past, or no row starts for %d rows of %d sequences", fn, n_tokens, n_seq);
     FL_TRY(ensure_device());
     AppendArgs a{};
@@ -95,7 +99,7 @@ static int fill(AttnArgs &a, const char *fn, int type, int head_dim, int n_head,
     if (n_head < 1 || n_head > 65535 || n_head % n_head_kv) return set_error(FL_EINVAL, "%s: %d query heads over %d key heads", fn, n_head, n_head_kv);
     if (!(scale > 0) || !std::isfinite(scale * 1.44269504088896341f)) return set_error(FL_EINVAL, "%s: scale %g is not a positive number", fn, (double)scale);
     if (n_seq < 0) return set_error(FL_EINVAL, "%s: %d sequences", fn, n_seq);
-    if ((int64_t)n_q * n_head > INT32_MAX) return set_error(FL_EINVAL, "%s: %d rows of %d heads: more than 2^31", fn, n_q, n_head);
+    if ((int64_t)n_q * n_head > MAX_COUNT) return set_error(FL_EINVAL, "%s: %d rows of %d heads: more than 2^31 - 512", fn, n_q, n_head);
     FL_TRY(check_heads(fn, "q", q, type, n_q));
     FL_TRY(check_out(fn, "out", out, type, n_q, n_head));
     a.q = q->data_dev, a.q_ld = q->token_stride, a.q_hs = q->head_stride;
@@ -123,6 +127,7 @@ int fl_attn_prompt(int type, int head_dim, int n_head, int n_head_kv, float scal
     FL_TRY(fill(a, fn, type, head_dim, n_head, n_head_kv, scale, q, out, n_q, n_seq));
     FL_TRY(check_heads(fn, "k", k, type, n_kv));
     FL_TRY(check_heads(fn, "v", v, type, n_kv));
+    if (n_kv > MAX_COUNT) return set_error(FL_EINVAL, "%s: %d keys: more than 2^31 - 512", fn, n_kv);
     if (n_q == 0 || n_seq == 0) return FL_OK;
     if (!cu_q_dev || !cu_kv_dev) return set_error(FL_EINVAL, "%s: null row starts", fn);
     FL_TRY(check_workspace(fn, "fl_attn_prompt_workspace", fl_attn_prompt_workspace(type, head_dim, n_head, n_head_kv, n_q, n_kv, n_seq), workspace_dev, workspace_bytes));

@@ -159,7 +159,8 @@ int fl_mul_mat_q_f32(const fl_qtensor *W, const float *x_dev, int ldx, float *y_
  *
  * Types: f32, f16, bf16; products, softmax statistics and sums are held in 32 bits (the sampler's in 64), outputs are rounded once.  In the
  * 16-bit types the softmax's numerators are rounded to the type before they meet the values (f16: below 2^-21 of the largest by up to 2^-32 of it).
- * Heads: query head h reads key head h / (n_head / n_head_kv).  head_dim: a multiple of 8 up to 128.  Data and strides are multiples of 16 bytes, rows at most 2^22 elements apart; the last axis is dense.
+ * Heads: query head h reads key head h / (n_head / n_head_kv).  head_dim: a multiple of 8 up to 128.  Data and strides are multiples of 16 bytes, rows at most
+ * 2^22 elements apart; the last axis is dense.  n_q * n_head and n_kv are at most 2^31 - 512, an append has at most 2^35 elements.
  *
  * Sequences: row starts `cu` (n_seq + 1 of them, not falling), lengths, past positions and page numbers are DEVICE data, so a captured graph
  * may be replayed on new ones.  Values that leave the buffers are cut, not reported: rows to those that exist, lengths to the table's
