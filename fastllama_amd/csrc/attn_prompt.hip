@@ -424,8 +424,10 @@ static hipError_t prompt_launch(const AttnArgs &a, int parts, hipStream_t st) {
 // Few workgroups (16-bit types): two waves for 32 rows.  A tile then takes a wave 1.3 us instead of 1.6, and there are twice as many workgroups: 512
 // rows behind 1536, 32 heads of 128 in f16 (128 blocks of 128 rows) 51 -> 42 us; 1000 rows, 32/8 heads in bf16 (256) 30 -> 27; but 2048, 32/32 (544)
 // 60 -> 64 and 4096, 32/8 (1032) 170 -> 202: each wave's share of a tile's loads and waits is as large as before.
-// Many: eight waves, which load a tile once for 256 rows: 8192 rows, 32/8 heads (1024 blocks of 256) 577 -> 542 us, 4096 (512) 174 -> 160; but 2048, 32/32
-// (256, one for each CU) 61 -> 68.
+// Many rows of long sequences: eight waves, which load a tile once for 256 rows.  8192 rows, 32/8 heads of 128 in bf16: 596 -> 555 us, 4096 in f16 178 -> 160,
+// two of 4096 316 -> 298; 2048, 32/32 in f16, as before (60).  With fewer than 2048 keys a sequence the last block's empty rows and the longest block's
+// way outweigh that: 16 of 512, 32/32 87 -> 95, 48 of 100 40 -> 58, 200 of 40 101 -> 160; four of 1024, 32/8 59 -> 57, eight packed ones of 1 to 1500
+// 61 either way.
 // Very few, behind many keys: the keys too are cut into parts of four tiles or more, until each CU has two workgroups, and joined by a second launch.  64
 // rows behind 30000, 32/8 heads of 128 in bf16: 575 -> 79 us (105 at one workgroup a CU); 16 behind 2000 in f16: 47 -> 20 (25 with parts of eight
 // tiles); 200 behind 1600, 8 heads in f32: 249 -> 44.  Where nearly each CU has one anyway, from 32 tiles on: 512 rows against 8192 keys, 32/32 in f16 (256
@@ -449,7 +451,7 @@ static hipError_t prompt_rows(const AttnArgs &a, hipStream_t st) {
     if constexpr (sizeof(T) == 2) {
         if (few_blocks(type, rows, n_head_kv, a.n_seq)) return prompt_launch<T, DP, PAGED, 2, 4>(a, parts, st);
         if constexpr (DP == 128 && !PAGED)
-            if (rows / 256 * n_head_kv >= 512) return prompt_launch<T, DP, PAGED, 1, 8>(a, 1, st);
+            if (rows / 256 * n_head_kv >= 512 && a.n_kv / 2048 >= a.n_seq) return prompt_launch<T, DP, PAGED, 1, 8>(a, 1, st);
     }
     return prompt_launch<T, DP, PAGED, 1, 4>(a, parts, st);
 }

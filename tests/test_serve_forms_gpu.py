@@ -27,10 +27,38 @@ def test_prompt_many_rows(ops, T, D, H, Hkv, pages):
 @pytest.mark.parametrize("T", [F16, BF16])
 @pytest.mark.parametrize("D", [72, 128])
 @pytest.mark.parametrize("H,Hkv,lens", [(256, 256, [1, 255, 257, 0, 40]), (512, 128, [1, 64, 65, 130]), (520, 104, [300, 1, 3])])
-def test_prompt_workgroups_of_256_rows(ops, T, D, H, Hkv, lens):
-    assert sum(lens) * (H // Hkv) // 256 * Hkv >= 512
+def test_prompt_many_rows_of_many_heads(ops, T, D, H, Hkv, lens):
     check_prompt(ops, T, H, Hkv, D, lens, lens, seed=D)
     check_prompt(ops, T, H, Hkv, D, lens, [n + 77 for n in lens], seed=D + 1)
+
+
+LONG = [(256, 256, [300, 1, 257], [2200, 2500, 2100]), (2048, 128, [64], [2048]), (320, 64, [450, 0, 30], [4000, 100, 2300])]
+
+
+@pytest.mark.parametrize("T", [F16, BF16])
+@pytest.mark.parametrize("D", [72, 128])
+@pytest.mark.parametrize("H,Hkv,lq,lk", LONG)
+def test_prompt_workgroups_of_256_rows(ops, T, D, H, Hkv, lq, lk):
+    """Many rows, 2048 keys a sequence and more."""
+    assert sum(lq) * (H // Hkv) // 256 * Hkv >= 512 and sum(lk) // 2048 >= len(lq)
+    check_prompt(ops, T, H, Hkv, D, lq, lk, seed=D)
+
+
+@pytest.mark.parametrize("T", [F16, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("at", [0, 5, 63, 64, 200, 299])
+def test_prompt_workgroups_of_256_rows_not_finite(ops, T, bad, at):
+    """A value that is not finite at the at-th new position of the first sequence: its rows from there on have it, nothing else does."""
+    H, Hkv, lq, lk = LONG[0]
+    q, k, v = randn(1, sum(lq), H, 128, dtype=T), randn(2, sum(lk), Hkv, 128, dtype=T), randn(3, sum(lk), Hkv, 128, dtype=T)
+    want = [attention64(q[a:a + m], k[b:b + n], v[b:b + n], 128 ** -0.5) for a, b, m, n in zip(np.cumsum([0] + lq), np.cumsum([0] + lk), lq, lk)]
+    v[lk[0] - lq[0] + at] = bad
+    got = ops.attn_prompt(q, k, v, starts(lq), starts(lk)).split(lq)
+    near(got[0][:at], want[0][0][:at], want[0][1][:at])
+    seen = got[0][at:].double()
+    assert (seen.isnan().all() if math.isnan(bad) else (seen == bad).all())
+    for g, (w, b) in zip(got[1:], want[1:]):
+        near(g, w, b)
 
 
 @pytest.mark.parametrize("T", [F16, BF16])
