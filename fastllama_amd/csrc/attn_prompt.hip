@@ -11,9 +11,10 @@
 // columns are query rows again: the rescaling factor is a lane's own.  V^T comes out of LDS by transposing reads.
 //
 // The softmax's reference is not the running maximum but a value at most 2^8 below it: the accumulators are rescaled only when the maximum
-// has moved by more.  p is rounded to the inputs' type for the second product (the error of a weighted mean of values that are themselves of that
-// type); scores, sums and outputs are f32 until the one rounding at the end.  f16 has p only down to 2^-24, so there it is taken 2^P_SHIFT times as large,
-// which cancels against the sum: p <= 2^15 still fits, and what is lost of a key is at most 2^-32 of the largest weight.
+// has moved by more.  p is rounded to the inputs' type for the second product, which the 16-bit matrix units ask for (the error of a weighted mean of
+// values that are themselves of that type: against 64 bits 0.0017 of the outputs' size in place of the 0.0016 of the last rounding alone in bf16, 0.00018
+// in place of 0.00017 in f16); scores, sums and outputs are f32 until the one rounding at the end.  f16 has p only down to 2^-24, so there it is
+// taken 2^P_SHIFT times as large, which cancels against the sum: p <= 2^15 still fits, and what is lost of a key is at most 2^-32 of the largest weight.
 #include "serve_kernels.h"
 #include "serve_device.h"
 #include "../../include/fastllama_hip.h"

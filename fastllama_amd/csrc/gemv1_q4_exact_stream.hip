@@ -391,8 +391,8 @@ static bool launch_stream(const fl_qtensor &W, const fl_qact *xq, float *y, hipS
     // Q4_0: four prologue-only waves in front of four streaming ones, where every workgroup has a CU of its own anyway (wq|wk|wv: 192 workgroups)
     // (more workgroups than CUs: two eight-wave workgroups per CU at 8 quads in flight, 122-128 registers)
     // Q4_1 goes without: it needs 130-134 registers at 8 quads in flight, and the 128 that four waves per SIMD leave spill 33-43 of them, some inside the
-    // streaming loop.  With / without those waves, ms per token: 7B 2.75 / 1.88, at n_past 2000 3.25 / 2.38, 13B 4.42 / 2.71, 65B 15.9 / 10.5; Q4_0 (122-126
-    // registers) 7B 1.572 / 1.640.
+    // streaming loop.  With / without those waves, ms per token: 7B 2.75 / 1.88, at n_past 2000 3.25 / 2.38, 13B 4.42 / 2.71, 65B 15.9 / 10.5 (before the
+    // waits in the kernel were written out; without, 1.81, 2.35, 2.66 and 10.3 since).  Q4_0 (122-126 registers) 7B 1.455 / 1.561.
     constexpr bool can_help = TYPE == FL_TYPE_Q4_0;
     if (can_help && g_stream_helpers && PRO == 1 && nw == 4 && (groups + 3) / 4 <= 2 * n_cus) maxw = 8;
     else if (can_help && g_stream_helpers && PRO == 1 && nw > 8) maxw = 16;      // (one workgroup per CU with up to twelve streaming waves: LLaMA-65B's w1|w3)

@@ -16,6 +16,8 @@ and the operators of a serving step over several sequences, which the reference 
 * ``attn_pages``           the same over a paged cache: one new token for each sequence, or chunks of prompts
 * ``sample``               temperature / top-k / top-p / min-p from given uniform numbers
 
+Inference only: no operator here records a gradient, also for tensors that require one.
+
 torch is used only to own device memory and to pick the stream; every computation happens inside
 libfastllama_hip.so.  Nothing here computes on the CPU.
 """

@@ -153,8 +153,9 @@ int fl_mul_mat_q(const fl_qtensor *W, const fl_qact *a, float *y_dev, int ldy, v
 int fl_mul_mat_q_f32(const fl_qtensor *W, const float *x_dev, int ldx, float *y_dev, int ldy, int N, void *stream);
 
 /* ---------------------------------------------------------------- several sequences -------------- */
-/* Operators of a serving step over several sequences (fl_mul_mat_q_f32 projects their rows; these do the rest): new keys and values go
- * into the pages of a cache, attention reads them, and a token is drawn for each row of logits.  New: the reference evaluates one
+/* The operators of a serving step that see several sequences: new keys and values go into the pages of a cache, attention reads them,
+ * and a token is drawn for each row of logits.  Products of rows are fl_mul_mat_q_f32; the norms, the rotation of q and k by their positions
+ * and the activation between the products are the caller's, and so is a repeat penalty on the logits.  New: the reference evaluates one
  * sequence, with the attention of lib/llama.cpp:344-399 and the sampler of lib/bridge.cpp:24-108.
  *
  * Types: f32, f16, bf16; products, softmax statistics and sums are held in 32 bits (the sampler's in 64), outputs are rounded once.  In the
