@@ -375,7 +375,7 @@ __global__ __launch_bounds__(64 * NK, (!PERSIST && QPW <= 8 && NK == 4) ? 3 : 1)
                         for (int blk = 0; blk < 4; ++blk) { msb[blk] = msb_[i][blk]; sxv[blk] = sxv_[i][blk]; }
                     } else if (Q41) {
                         // (m_w of a block sits in one lane of the row's quad, as d_w does; broadcast here, in the chain -- kept as four registers
-                        //  per quad since the order-free part it cost Q4_1 its third workgroup per CU: round 5)
+                        //  per quad since the order-free part it cost Q4_1 its third workgroup per CU)
                         msb[0] = quad_bcast<0>(mw[i]); msb[1] = quad_bcast<1>(mw[i]); msb[2] = quad_bcast<2>(mw[i]); msb[3] = quad_bcast<3>(mw[i]);
                         const float4 sx4 = *reinterpret_cast<const float4 *>(ls_ + 4 * (qlo + i));
                         sxv[0] = sx4.x; sxv[1] = sx4.y; sxv[2] = sx4.z; sxv[3] = sx4.w;
